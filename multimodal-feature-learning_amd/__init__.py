@@ -61,6 +61,7 @@ from .models.ops.modules import ms_deform_attn  # noqa: E402,F401
 from . import utils  # noqa: E402,F401
 from .utils import dam, box_ops, preds_postprocess  # noqa: E402,F401
 from .models import matcher, load_weights, dvc_common  # noqa: E402,F401
+from .models.modules import paged_cache, logits  # noqa: E402,F401
 from .models.modules import layers  # noqa: E402,F401
 from .models import unimodal_caption_decoder, multimodal_caption_decoder  # noqa: E402,F401
 from .models.deformable import unimodal_deformable_dvc, multimodal_deformable_dvc  # noqa: E402,F401

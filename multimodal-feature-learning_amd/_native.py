@@ -5,6 +5,7 @@ library is missing or fails to load, every MSDA call raises ``RuntimeError`` (th
 reference's native op likewise raises ``AT_ERROR("Not implemented on the CPU")`` for
 CPU tensors, models/ops/src/cpu/ms_deform_attn_cpu.cpp:17-41).
 """
+import contextlib
 import ctypes
 import os
 import threading
@@ -103,6 +104,21 @@ EXPORTED_SYMBOLS = (
     "mfl_lsa_levels",
     "msda_hip_last_error",
     "msda_hip_abi_version",
+)
+
+# include/paged_cache.h and include/logits_process.h (caption serving, same library)
+SERVING_SYMBOLS = (
+    "mfl_paged_attention_workspace_bytes",
+    "mfl_paged_attention",
+    "mfl_pages_update_workspace_bytes",
+    "mfl_pages_update",
+    "mfl_pages_compact_workspace_bytes",
+    "mfl_pages_compact",
+    "mfl_pages_copy",
+    "mfl_paged_last_error",
+    "mfl_logits_workspace_bytes",
+    "mfl_logits_process",
+    "mfl_logits_last_error",
 )
 
 _lock = threading.Lock()
@@ -272,6 +288,30 @@ def _declare(lib):
     lib.msda_hip_last_error.argtypes = []
     lib.msda_hip_abi_version.restype = i32
     lib.msda_hip_abi_version.argtypes = []
+    # (argument structs: passed as the packed bytes of include/paged_cache.h's / logits_process.h's fields)
+    raw = ctypes.c_char_p
+    lib.mfl_paged_attention_workspace_bytes.restype = i64
+    lib.mfl_paged_attention_workspace_bytes.argtypes = [raw]
+    lib.mfl_paged_attention.restype = i32
+    lib.mfl_paged_attention.argtypes = [raw, vp]
+    lib.mfl_pages_update_workspace_bytes.restype = i64
+    lib.mfl_pages_update_workspace_bytes.argtypes = [i64, i64]
+    lib.mfl_pages_update.restype = i32
+    lib.mfl_pages_update.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i64, vp, i64, i64, i64, vp, vp, vp, vp, vp, vp]
+    lib.mfl_pages_compact_workspace_bytes.restype = i64
+    lib.mfl_pages_compact_workspace_bytes.argtypes = [i64]
+    lib.mfl_pages_compact.restype = i32
+    lib.mfl_pages_compact.argtypes = [vp, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp]
+    lib.mfl_pages_copy.restype = i32
+    lib.mfl_pages_copy.argtypes = [vp, vp, i64, vp, i64, i64, i64, vp]
+    lib.mfl_paged_last_error.restype = ctypes.c_char_p
+    lib.mfl_paged_last_error.argtypes = []
+    lib.mfl_logits_workspace_bytes.restype = i64
+    lib.mfl_logits_workspace_bytes.argtypes = [raw]
+    lib.mfl_logits_process.restype = i32
+    lib.mfl_logits_process.argtypes = [raw, vp]
+    lib.mfl_logits_last_error.restype = ctypes.c_char_p
+    lib.mfl_logits_last_error.argtypes = []
     lib.mfl_lsa.restype = i32
     lib.mfl_lsa.argtypes = [vp, i64, i64, vp, vp]
     lib.mfl_lsa_levels.restype = i32
@@ -317,6 +357,16 @@ def host_i64_array(values):
 
 def stream_handle(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_same_device = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context in which ``device`` is the current one (kernels launch on the current device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _same_device
+    return torch.cuda.device(device)
 
 
 _own_streams = {}

@@ -1,0 +1,286 @@
+"""Paged attention (csrc/paged_attention.hip) against the 64-bit form of oracle/serving_oracle.py.
+
+Tolerance, elementwise, with u = eps / 2 of the type (a rounding is off by at most half a step) and, over the row's visible
+keys, A = sum_j p_j |v_j|, S = max_j scale sum_d |q_d k_jd|:
+  u |out|                       the output's rounding
+  u A                           the weights' rounding to the values' type before the matrix product (16-bit types)
+  2 w A, w = (D + 8) 2^-24 S + 2^-20   the weights' relative error, in numerator and denominator: fp32 dot products of D
+                                terms, the scaled difference and the exponential (2^-20 covers its few ulp and
+                                the rescales)
+  2 K 2^-24 A                   fp32 sums over K keys
+  2^-25 sum_j |v_j|             fp16 only: weights below its smallest normal number, rounded to its steps of 2^-24
+                                (the largest weight is 1, so the denominator is at least 1)
+"""
+import pytest
+import torch
+
+from conftest import PKG
+from oracle import serving_oracle as O
+
+pytestmark = pytest.mark.gpu
+pc = PKG.models.modules.paged_cache
+BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def tolerance(ref, aux, dtype, dim, keys):
+    u = torch.finfo(dtype).eps / 2
+    A, V, S = aux
+    w = (dim + 8) * 2.0 ** -24 * S[..., None] + 2.0 ** -20
+    tol = u * ref.abs() + (u if dtype != F32 else 0.0) * A + 2 * w * A + 2 * keys * 2.0 ** -24 * A
+    if dtype == FP:
+        tol = tol + 2.0 ** -25 * V
+    return tol + 1e-30
+
+
+def make(n, rows, heads, kvh, dim, ps, kv, dtype, seed, packed=None, write=False, starts=None, spare=2):
+    """CPU inputs: shuffled pages, NaN in every cell that belongs to no sequence's visible tokens."""
+    g = torch.Generator().manual_seed(seed)
+    need = [(max(v, 0) + ps - 1) // ps for v in kv]
+    width = max(need + [1]) + 1
+    pages = sum(need) + spare
+    order = torch.randperm(pages, generator=g).tolist()
+    table = torch.full((n, width), -1, dtype=torch.int32)
+    live = torch.zeros(pages, ps, dtype=torch.bool)
+    at = 0
+    for s, m in enumerate(need):
+        for c in range(m):
+            table[s, c] = order[at]
+            live[order[at], :max(0, min(ps, kv[s] - c * ps))] = True
+            at += 1
+    kp = torch.randn(pages, kvh, ps, dim, generator=g).to(dtype)
+    vp = torch.randn(pages, kvh, ps, dim, generator=g).to(dtype)
+    dead = ~live[:, None, :, None].expand_as(kp)
+    kp[dead] = float("nan")
+    vp[dead] = float("nan")
+    lead = (n, rows) if packed is None else (packed[-1] + 3,)
+    q = (torch.randn(*lead, heads, dim, generator=g) * 1.5).to(dtype)
+    k = torch.randn(*lead, kvh, dim, generator=g).to(dtype) if write else None
+    v = torch.randn(*lead, kvh, dim, generator=g).to(dtype) if write else None
+    i32 = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    return dict(q=q, k_pages=kp, v_pages=vp, table=table, kv_lens=i32(kv), k=k, v=v, starts=i32(starts),
+                offsets=i32(packed))
+
+
+def up(d, dev):
+    return {k: (t.to(dev) if isinstance(t, torch.Tensor) else t) for k, t in d.items()}
+
+
+def call(d, **kw):
+    d = dict(d)
+    return pc.paged_attention(d.pop("q"), d.pop("k_pages"), d.pop("v_pages"), d.pop("table"), d.pop("kv_lens"), **d, **kw)
+
+
+def check(out, d, kp=None, vp=None, **kw):
+    ref, aux, rk, rv = O.paged_attention(**d, **kw)
+    tol = tolerance(ref, aux, d["q"].dtype, d["q"].shape[-1], int(d["kv_lens"].max()))
+    err = (out.double().cpu() - ref).abs()
+    bad = ~(err <= tol)
+    assert not bool(bad.any()), (int(bad.sum()), float((err / tol)[bad].max()), bad.nonzero()[:4].tolist())
+    if kp is not None:  # the pages, cell for cell (NaN where nothing is)
+        assert torch.equal(kp.cpu().nan_to_num(7.25), rk.nan_to_num(7.25))
+        assert torch.equal(vp.cpu().nan_to_num(7.25), rv.nan_to_num(7.25))
+
+
+CASES = [
+    # n, rows, heads, kv_heads, dim, page, kv
+    (3, 1, 4, 4, 64, 16, [1, 17, 0]),              # single tokens, an empty sequence
+    (4, 2, 8, 8, 64, 16, [2, 19, 31, 33]),         # token + probe
+    (2, 1, 8, 1, 128, 8, [300, 1]),                # eight heads of one key head, split along the keys
+    (2, 3, 12, 4, 32, 1, [40, 5]),                 # one-token pages
+    (2, 5, 6, 2, 96, 64, [200, 64]),               # dim between tiles
+    (1, 20, 12, 12, 40, 32, [45]),                 # dim 40, one row tile per head
+    (2, 70, 4, 2, 64, 16, [70, 131]),              # many rows: the shared-tile kernel
+    (1, 150, 8, 1, 128, 128, [1000]),
+    (2, 90, 3, 3, 8, 4, [95, 90]),                 # dim 8
+    (1, 33, 8, 8, 128, 16, [2049]),                # two row tiles, key ranges
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"r{c[1]}_h{c[2]}x{c[3]}_d{c[4]}_p{c[5]}")
+def test_matches_64_bit(dev, case, dtype):
+    n, rows, heads, kvh, dim, ps, kv = case
+    d = make(n, rows, heads, kvh, dim, ps, kv, dtype, seed=rows * 7 + dim)
+    g = up(d, dev)
+    check(call(g), d)
+    check(call(g, max_kv=max(kv)), d)
+    check(call(g, causal=False, scale=0.3), d, causal=False, scale=0.3)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"r{c[1]}_h{c[2]}x{c[3]}_d{c[4]}_p{c[5]}")
+def test_writes_the_chunk(dev, case, dtype):
+    """The chunk's own rows are written (also those the pages hold NaN for), read, and nothing else is touched."""
+    n, rows, heads, kvh, dim, ps, kv = case
+    d = make(n, rows, heads, kvh, dim, ps, kv, dtype, seed=rows * 11 + dim, write=True)
+    g = up(d, dev)
+    check(call(g), d, g["k_pages"], g["v_pages"])
+
+
+@pytest.mark.parametrize("write", [False, True])
+@pytest.mark.parametrize("max_rows", [None, 40])
+def test_packed_rows(dev, write, max_rows):
+    """Packed chunks of 0, 1, 33 and 40 rows; the rows behind the last sequence are 0, or left as they were."""
+    packed = [0, 0, 1, 34, 74]
+    d = make(4, 0, 8, 2, 64, 16, [9, 50, 33, 301], BF, 5, packed=packed, write=write)
+    g = up(d, dev)
+    out = call(g, max_rows=max_rows)
+    check(out, d, g["k_pages"], g["v_pages"])
+    assert bool((out[74:] == 0).all())
+    mine = torch.full_like(out, 3.0)
+    call(g, max_rows=max_rows, out=mine)
+    assert torch.equal(mine[:74], out[:74]) and bool((mine[74:] == 3).all())
+
+
+def test_packed_offsets_out_of_range_are_clamped(dev):
+    d = make(2, 0, 4, 4, 64, 16, [30, 30], BF, 6, packed=[0, 5, 11])
+    d["offsets"] = torch.tensor([0, 5, 1000], dtype=torch.int32)  # q has 14 rows
+    g = up(d, dev)
+    out = call(g)
+    d["offsets"] = torch.tensor([0, 5, 14], dtype=torch.int32)
+    d["starts"] = torch.tensor([25, 30 - 9], dtype=torch.int32)
+    check(out, d)
+
+
+@pytest.mark.parametrize("rows, dtype", [(2, BF), (2, F32), (80, BF), (80, F32)])
+def test_starts(dev, rows, dtype):
+    """Rows before the first key, a probe behind the last, far positions, a chunk inside the cache."""
+    kv = [40, 41, 42, 150, 40]
+    starts = [-3, 41 - 1, 2 ** 31 - 5, 20, -2 ** 31]
+    d = make(5, rows, 4, 2, 64, 16, kv, dtype, 8, write=True, starts=starts)
+    g = up(d, dev)
+    out = call(g)
+    check(out, d, g["k_pages"], g["v_pages"])
+    assert bool((out[0, :3] == 0).all()) and bool((out[4] == 0).all())
+
+
+@pytest.mark.parametrize("rows", [1, 80])
+def test_bad_pages_and_lens_are_not_read(dev, rows):
+    """Page numbers outside the pool hide their keys; lengths beyond the table are cut to it."""
+    d = make(3, rows, 4, 2, 64, 16, [100, 90, 85], BF, 9, write=True)
+    d["table"][0, 2] = -1
+    d["table"][1, 0] = 10 ** 9
+    d["table"][2, :] = -7
+    d["kv_lens"][1] = 2 ** 30
+    d["starts"] = torch.tensor([100 - rows, 90 - rows, 85 - rows], dtype=torch.int32)
+    g = up(d, dev)
+    d["k_pages"], d["v_pages"] = d["k_pages"].nan_to_num(0.5), d["v_pages"].nan_to_num(0.5)
+    g["k_pages"], g["v_pages"] = d["k_pages"].to(dev), d["v_pages"].to(dev)
+    out = call(g)
+    check(out, d, g["k_pages"], g["v_pages"])
+    assert bool((out[2] == 0).all())
+
+
+@pytest.mark.parametrize("rows", [2, 70])
+def test_strided_and_misaligned_inputs(dev, rows):
+    d = make(2, rows, 4, 2, 64, 16, [80, 75], BF, 10, write=True)
+    g = up(d, dev)
+    want = call({**g, "k_pages": g["k_pages"].clone(), "v_pages": g["v_pages"].clone()})
+    t = dict(g)
+    for nm in ("q", "k", "v"):
+        x = g[nm]
+        t[nm] = x.transpose(1, 2).contiguous().transpose(1, 2)       # head-major storage
+        assert not t[nm].is_contiguous()
+    assert torch.equal(call({**t, "k_pages": g["k_pages"].clone(), "v_pages": g["v_pages"].clone()}), want)
+    for nm in ("q", "k", "v"):
+        x = torch.empty(g[nm].numel() + 3, dtype=BF, device=dev)[3:].view(g[nm].shape)  # 6 bytes off
+        x.copy_(g[nm])
+        t[nm] = x
+    assert torch.equal(call({**t, "k_pages": g["k_pages"].clone(), "v_pages": g["v_pages"].clone()}), want)
+
+
+def test_non_finite_values(dev):
+    """A NaN query spoils its own row; NaN or infinite keys and values behind a sequence's length nothing."""
+    d = make(2, 2, 4, 4, 64, 16, [20, 9], BF, 11)
+    g = up(d, dev)
+    clean = call(g)
+    dead = g["k_pages"].isnan()
+    for bad in (float("inf"), float("-inf")):
+        h = dict(g)
+        h["k_pages"], h["v_pages"] = g["k_pages"].clone(), g["v_pages"].clone()
+        h["k_pages"][dead], h["v_pages"][dead] = bad, bad
+        assert torch.equal(call(h), clean)
+    h = dict(g, q=g["q"].clone())
+    h["q"][0, 1, 2] = float("nan")
+    out = call(h)
+    assert bool(out[0, 1, 2].isnan().all())
+    keep = torch.ones(out.shape[:-1], dtype=torch.bool, device=dev)
+    keep[0, 1, 2] = False
+    assert torch.equal(out[keep], clean[keep])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_infinite_value_of_a_later_token_stays_out_of_earlier_rows(dev, dtype):
+    """A chunk's token with an infinite value reaches the rows that see it, and no row before it."""
+    for rows in (3, 80):
+        d = make(1, rows, 4, 2, 64, 16, [rows + 6], dtype, 12, write=True)
+        g = up(d, dev)
+        clean = call({**g, "k_pages": g["k_pages"].clone(), "v_pages": g["v_pages"].clone()})
+        at = rows // 2
+        v = g["v"].clone()
+        v[0, at, 0, 5] = float("inf")
+        out = call({**g, "v": v, "k_pages": g["k_pages"].clone(), "v_pages": g["v_pages"].clone()})
+        assert torch.equal(out[0, :at], clean[0, :at])
+        assert bool(torch.isinf(out[0, at:, 0, 5]).all()) and bool(torch.isinf(out[0, at:, 1, 5]).all())
+
+
+def test_offsets_past_32_bits(dev):
+    """Pages whose byte offsets pass 2^32 and element offsets 2^31."""
+    kvh, ps, dim = 8, 64, 128
+    pages = 2 ** 31 // (kvh * ps * dim) + 40
+    kp = torch.empty(pages, kvh, ps, dim, dtype=BF, device=dev)
+    vp = torch.empty(pages, kvh, ps, dim, dtype=BF, device=dev)
+    d = make(2, 1, 16, 8, 128, 64, [200, 70], BF, 13, write=True)
+    g = up(d, dev)
+    far = torch.arange(pages - d["k_pages"].shape[0], pages, device=dev)
+    kp[far], vp[far] = g["k_pages"], g["v_pages"]
+    table = torch.where(g["table"] >= 0, g["table"] + int(far[0]), g["table"])
+    out = call({**g, "k_pages": kp, "v_pages": vp, "table": table.to(torch.int32)})
+    check(out, d, kp[far], vp[far])
+
+
+def test_long_cache_split(dev):
+    """One row over 30,001 keys: many key ranges joined; and the same through a wrong (small) max_kv."""
+    d = make(1, 1, 4, 1, 64, 32, [30001], BF, 14)
+    g = up(d, dev)
+    check(call(g), d)
+    check(call(g, max_kv=16), d)
+
+
+def test_other_stream_and_graph(dev):
+    d = make(3, 2, 8, 2, 128, 16, [900, 1200, 3], BF, 15, write=True)
+    g = up(d, dev)
+    want = call(g)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = call(g)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+    graphs = []
+    for _ in range(2):  # two graphs: their workspaces are their own
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = call(g)
+        graphs.append((gr, out))
+    for it in range(3):
+        g["q"].copy_(up(make(3, 2, 8, 2, 128, 16, [900, 1200, 3], BF, 20 + it, write=True), dev)["q"])
+        eager = call(g)
+        for gr, out in graphs:
+            out.zero_()
+            gr.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert torch.equal(out, eager)
+
+
+def test_empty_calls(dev):
+    d = up(make(2, 1, 4, 2, 64, 16, [5, 6], BF, 16), dev)
+    assert call({**d, "q": d["q"][:, :0]}).shape == (2, 0, 4, 64)
+    z = {**d, "q": d["q"][:0], "table": d["table"][:0], "kv_lens": d["kv_lens"][:0]}
+    assert call(z).shape == (0, 1, 4, 64)
+    one = torch.ones(3, 4, 64, dtype=BF, device=dev)  # no sequence at all: every packed row is behind the last
+    off = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = call({**z, "q": one, "offsets": off})
+    assert bool((out == 0).all())
+    assert bool((call({**d, "kv_lens": torch.zeros_like(d["kv_lens"])}) == 0).all())

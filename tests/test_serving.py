@@ -1,0 +1,212 @@
+"""Caption serving without a GPU: the headers against the binding, and the refusals of the entry points (in
+Python before anything touches a device, in the C-ABI before a launch)."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+from conftest import PKG, ROOT
+
+nat = PKG._native
+pc = PKG.models.modules.paged_cache
+lg = PKG.models.modules.logits
+
+
+def test_header_symbols_match_binding_and_library():
+    names = set()
+    for h in ("paged_cache.h", "logits_process.h"):
+        text = open(os.path.join(ROOT, "include", h)).read()
+        names |= set(re.findall(r"^(?:const\s+)?[a-z_0-9]+\s*\*?\s*(mfl_\w+)\s*\(", text, re.M))
+    assert sorted(names) == sorted(nat.SERVING_SYMBOLS)
+    lib = ctypes.CDLL(nat.LIB_PATH)
+    for name in names:
+        assert hasattr(lib, name), name
+
+
+# --- paged attention --------------------------------------------------------------------------------
+
+def _att(**kw):
+    a = dict(q=torch.zeros(2, 3, 4, 64), k_pages=torch.zeros(5, 2, 16, 64), v_pages=torch.zeros(5, 2, 16, 64),
+             table=torch.zeros(2, 2, dtype=torch.int32), kv_lens=torch.zeros(2, dtype=torch.int32))
+    a.update(kw)
+    return pc.paged_attention(a.pop("q"), a.pop("k_pages"), a.pop("v_pages"), a.pop("table"), a.pop("kv_lens"), **a)
+
+
+def _i(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("err, kw", [
+    (TypeError, dict(q=torch.zeros(2, 3, 4, 64, dtype=torch.float64))),
+    (TypeError, dict(k_pages=torch.zeros(5, 2, 16, 64, dtype=torch.bfloat16))),
+    (TypeError, dict(table=torch.zeros(2, 2, dtype=torch.int64))),
+    (TypeError, dict(kv_lens=torch.zeros(2, dtype=torch.int64))),
+    (TypeError, dict(starts=torch.zeros(2))),
+    (ValueError, dict(q=torch.zeros(2, 3, 4, 32))),
+    (ValueError, dict(q=torch.zeros(2, 3, 3, 64))),
+    (ValueError, dict(q=torch.zeros(6, 4, 64))),
+    (ValueError, dict(q=torch.zeros(3, 3, 4, 64))),
+    (ValueError, dict(v_pages=torch.zeros(4, 2, 16, 64))),
+    (ValueError, dict(k_pages=torch.zeros(5, 16, 2, 64).transpose(1, 2))),
+    (ValueError, dict(k=torch.zeros(2, 3, 2, 64))),
+    (ValueError, dict(k=torch.zeros(2, 3, 4, 64), v=torch.zeros(2, 3, 4, 64))),
+    (ValueError, dict(kv_lens=_i(3))),
+    (ValueError, dict(table=_i(2))),
+    (ValueError, dict(offsets=_i(3))),
+    (ValueError, dict(q=torch.zeros(6, 4, 64), offsets=_i(2))),
+    (ValueError, dict(q=torch.zeros(6, 4, 64), offsets=_i(3), max_rows=-1)),
+    (ValueError, dict(out=torch.zeros(2, 3, 4, 32))),
+    (RuntimeError, dict(q=torch.zeros(2, 3, 4, 64, requires_grad=True))),
+    (RuntimeError, dict()),  # host tensors: there is no CPU implementation
+])
+def test_attention_refuses(err, kw):
+    with pytest.raises(err):
+        _att(**kw)
+
+
+def _att_args(**kw):
+    f = dict(q=16, kn=0, vn=0, kp=16, vp=16, out=16, ws=16, table=16, kv_lens=16, starts=0, offsets=0, n=2, rows=3,
+             total=0, heads=4, kv_heads=2, dim=64, pages=5, page_size=16, width=2, max_kv=32, q_seq=768, q_row=256,
+             q_head=64, k_seq=0, k_row=0, k_head=0, v_seq=0, v_row=0, v_head=0, dtype=2, causal=1, zero_tail=0,
+             scale=0.125)
+    f.update(kw)
+    return pc._ARGS.pack(*f.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=1), dict(dtype=9), dict(n=-1), dict(rows=-1), dict(heads=3), dict(kv_heads=0), dict(dim=0), dict(dim=136),
+    dict(dim=4), dict(dim=60), dict(page_size=0), dict(page_size=24), dict(page_size=2048), dict(scale=0.0),
+    dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(kn=16), dict(q_row=3), dict(q=8),
+    dict(kp=24), dict(width=1 << 27), dict(rows=1 << 31), dict(q=0), dict(table=0), dict(kv_lens=0),
+    dict(n=1 << 30, rows=1 << 20), dict(ws=0, max_kv=1 << 20, width=1 << 16, rows=1), dict(pages=1 << 31)])
+def test_attention_c_abi_refuses(kw):
+    lib = nat.load_library()
+    assert lib.mfl_paged_attention(_att_args(**kw), None) == 1
+    assert b"mfl_paged_attention" in lib.mfl_paged_last_error()
+
+
+def test_attention_c_abi_empty_calls_and_workspace():
+    lib = nat.load_library()
+    assert lib.mfl_paged_attention(_att_args(n=0), None) == 0
+    assert lib.mfl_paged_attention(_att_args(rows=0), None) == 0
+    assert lib.mfl_paged_attention(None, None) == 1
+    assert lib.mfl_paged_attention_workspace_bytes(_att_args(dim=60)) == -1
+    assert lib.mfl_paged_attention_workspace_bytes(_att_args()) == 0
+    assert lib.mfl_paged_attention_workspace_bytes(_att_args(rows=1, width=1 << 16, max_kv=1 << 20)) > 0
+
+
+# --- pages -------------------------------------------------------------------------------------------
+
+def _upd(**kw):
+    a = dict(data=torch.zeros(1, 2, 6, 2, 16, 8), table=_i(3, 2), lens=_i(3), refs=_i(6))
+    a.update(kw)
+    return pc.pages_update(a.pop("data"), a.pop("table"), a.pop("lens"), a.pop("refs"), **a)
+
+
+@pytest.mark.parametrize("err, kw", [
+    (TypeError, dict(table=torch.zeros(3, 2))), (TypeError, dict(lens=torch.zeros(3, dtype=torch.int64))),
+    (TypeError, dict(parents=torch.zeros(3, dtype=torch.int64))), (ValueError, dict(table=_i(3))),
+    (ValueError, dict(lens=_i(2))), (ValueError, dict(refs=_i(5))), (ValueError, dict(refs=_i(6, 1))),
+    (ValueError, dict(new_lens=_i(4))), (ValueError, dict(data=torch.zeros(2, 6, 2, 16, 8))),
+    (ValueError, dict(data=torch.zeros(1, 2, 6, 2, 16, 3))), (ValueError, dict(page_size=8)),
+    (ValueError, dict(data=None)), (RuntimeError, dict())])
+def test_update_refuses(err, kw):
+    with pytest.raises(err):
+        _upd(**kw)
+
+
+@pytest.mark.parametrize("err, kw", [
+    (TypeError, dict(refs=torch.zeros(6))), (TypeError, dict(table=torch.zeros(3, 2))),
+    (ValueError, dict(refs=_i(5))), (ValueError, dict(refs=_i(2, 3))), (RuntimeError, dict())])
+def test_compact_refuses(err, kw):
+    a = dict(data=torch.zeros(1, 2, 6, 2, 16, 8), table=_i(3, 2), refs=_i(6))
+    a.update(kw)
+    with pytest.raises(err):
+        pc.pages_compact(a["data"], a["table"], a["refs"])
+
+
+@pytest.mark.parametrize("err, kw", [
+    (TypeError, dict(src=torch.zeros(2))), (ValueError, dict(dst=_i(3))), (ValueError, dict(src=_i(2, 1))),
+    (ValueError, dict(data=None)), (RuntimeError, dict())])
+def test_copy_refuses(err, kw):
+    a = dict(data=torch.zeros(1, 2, 6, 2, 16, 8), src=_i(2), dst=_i(2))
+    a.update(kw)
+    with pytest.raises(err):
+        pc.pages_copy(a["data"], a["src"], a["dst"])
+
+
+def test_pages_c_abi_refuses():
+    lib = nat.load_library()
+    p = ctypes.c_void_p(16)  # never dereferenced
+    good = [p, p, p, None, None, 3, 2, 6, 16, p, 2, 2, 64, p, p, p, p, p, None]
+    for at, val in [(5, -1), (5, 1 << 21), (6, -1), (7, -1), (7, 1 << 31), (8, 0), (8, 24), (8, 2048), (10, 0), (11, 0),
+                    (12, 8), (12, 24), (9, ctypes.c_void_p(24)), (0, None), (1, None), (2, None), (13, None), (14, None),
+                    (15, None), (16, None), (17, None), (6, 1 << 28)]:
+        a = list(good)
+        a[at] = val
+        assert lib.mfl_pages_update(*a) == 1, (at, val)
+        assert b"mfl_pages_update" in lib.mfl_paged_last_error()
+    good = [p, 6, p, 6, p, 2, 1024, p, p, p, p, p, None]
+    for at, val in [(0, None), (1, -1), (2, None), (3, -1), (5, 0), (6, 8), (6, 0), (7, None), (8, None), (9, None),
+                    (10, None), (11, None)]:
+        a = list(good)
+        a[at] = val
+        assert lib.mfl_pages_compact(*a) == 1, (at, val)
+    good = [p, p, 2, p, 2, 6, 1024, None]
+    for at, val in [(0, None), (1, None), (2, -1), (3, None), (4, 0), (5, -1), (6, 24)]:
+        a = list(good)
+        a[at] = val
+        assert lib.mfl_pages_copy(*a) == 1, (at, val)
+    assert lib.mfl_pages_copy(p, p, 0, p, 2, 6, 1024, None) == 0
+    assert lib.mfl_pages_update_workspace_bytes(-1, 4) == -1 and lib.mfl_pages_compact_workspace_bytes(-1) == -1
+
+
+def test_cache_refuses_page_size():
+    with pytest.raises(ValueError):
+        pc.PagedKVCache(1, 2, 20, 2, 64, page_size=12, device="cpu")
+
+
+# --- logits ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("err, kw", [
+    (TypeError, dict(logits=torch.zeros(2, 40, dtype=torch.float64))), (ValueError, dict(logits=torch.zeros(40))),
+    (ValueError, dict(logits=torch.zeros(2, 0))), (TypeError, dict(tokens=torch.zeros(2, 3, dtype=torch.int64))),
+    (ValueError, dict(tokens=_i(3, 3))), (ValueError, dict(token_lens=_i(2))),
+    (ValueError, dict(tokens=_i(2, 3), token_lens=_i(3))), (ValueError, dict(repetition=0.0)),
+    (ValueError, dict(repetition=float("nan"))), (ValueError, dict(repetition=torch.ones(3))),
+    (ValueError, dict(presence=torch.ones(2, dtype=torch.float64))), (TypeError, dict(bias=torch.zeros(40).bfloat16())),
+    (ValueError, dict(bias=torch.zeros(41))), (TypeError, dict(allowed=torch.zeros(40))),
+    (ValueError, dict(allowed=torch.ones(41, dtype=torch.bool))), (ValueError, dict(allowed=_i(3))),
+    (ValueError, dict(allowed=torch.ones(3, 40, dtype=torch.bool))), (ValueError, dict(states=_i(2))),
+    (ValueError, dict(allowed=_i(3, 2), states=_i(3))), (ValueError, dict(out=torch.zeros(2, 41))),
+    (RuntimeError, dict(logits=torch.zeros(2, 40, requires_grad=True))), (RuntimeError, dict())])
+def test_logits_refuse(err, kw):
+    kw = dict(kw)
+    x = kw.pop("logits", torch.zeros(2, 40))
+    with pytest.raises(err):
+        lg.process_logits(x, **kw)
+    if "out" not in kw:
+        with pytest.raises(err):
+            lg.pick_tokens(x, **kw)
+
+
+def _lg_args(**kw):
+    f = dict(logits=16, out=32, best=16, lse=16, logprob=0, tokens=16, token_lens=0, rep=0, pres=0, freq=0, bias=0,
+             allowed=0, states=0, ws=16, n=2, vocab=40, dtype=0, out_dtype=0, logits_row=40, out_row=40, hist=3,
+             tokens_row=3, bias_row=0, kind=0, allowed_row=0, allowed_rows=0, repetition=1.0, presence=0.0, frequency=0.0)
+    f.update(kw)
+    return lg._ARGS.pack(*f.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n=-1), dict(vocab=-1), dict(vocab=0), dict(hist=-1), dict(dtype=1), dict(out_dtype=1), dict(kind=3),
+    dict(kind=1, allowed=16, allowed_rows=0), dict(kind=1, allowed=16, allowed_rows=3, allowed_row=39),
+    dict(kind=1, allowed=0, allowed_rows=1), dict(repetition=0.0), dict(out=16, out_dtype=2), dict(logits=0),
+    dict(tokens=0), dict(out_row=39), dict(vocab=100000, out_row=100000, ws=0), dict(n=1 << 23, vocab=1 << 30)])
+def test_logits_c_abi_refuses(kw):
+    lib = nat.load_library()
+    assert lib.mfl_logits_process(_lg_args(**kw), None) == 1
+    assert b"mfl_logits_process" in lib.mfl_logits_last_error()
+    assert lib.mfl_logits_process(None, None) == 1
