@@ -26,8 +26,8 @@ import torch
 from torch import nn
 
 from ..base_encoder import build_base_encoder
-from ..dvc_common import append_end_token, context_mask, look_ahead_mask, make_padding_mask, segment_memory, \
-    special_tokens
+from ..dvc_common import append_end_token, context_mask, decode_captions, look_ahead_mask, make_padding_mask, \
+    segment_memory, special_tokens
 from ..modules.embedding_layers import PositionEmbeddingVideoSine
 from ..modules.layers import FFN, ContextMaskModel
 from ..modules.linear import Linear
@@ -40,6 +40,9 @@ __all__ = ["MultimodalDeformableDVC"]
 
 
 class MultimodalDeformableDVC(nn.Module):
+    # inference: None — the greedy decode; a dict — options of the caption decoder's ``generate``
+    caption_options = None
+
     def __init__(self, input_modalities, num_queries, d_model, num_classes, aux_loss, matcher, threshold,
                  max_eseq_length=10, vocab=None, seq_len=None, embedding_matrix=None, detr_args=None, caption_args=None,
                  use_differentiable_mask=False, sparse_detr_args=None):
@@ -173,8 +176,8 @@ class MultimodalDeformableDVC(nn.Module):
 
         bos, eos, pad = special_tokens(self.vocab)
         (v_mem, _, v_key), (a_mem, _, a_key) = vids[-1], auds[-1]
-        captions, last_input = self.multimodal_caption_decoder.greedy_decode(v_mem, v_key, a_mem, a_key, bos, eos, pad,
-                                                                             self.seq_len - 1, faster_eval)
+        captions, last_input = decode_captions(self.multimodal_caption_decoder, (v_mem, v_key, a_mem, a_key), self.vocab,
+                                               self.seq_len - 1, faster_eval, self.caption_options)
         out['pred_captions'] = self._caption_probs(last_input, vids[-1], auds[-1])
         captions_with_eos = append_end_token(captions, self.vocab, faster_eval)
         indices_aux = []

@@ -24,8 +24,8 @@ import torch
 from torch import nn
 
 from ..base_encoder import build_base_encoder
-from ..dvc_common import (append_end_token, context_mask, make_padding_mask, make_tgt_mask, segment_memory,
-                          special_tokens)
+from ..dvc_common import (append_end_token, context_mask, decode_captions, make_padding_mask, make_tgt_mask,
+                          segment_memory, special_tokens)
 from ..modules.embedding_layers import PositionEmbeddingVideoSine
 from ..modules.layers import FFN, ContextMaskModel
 from ..modules.linear import Linear
@@ -38,6 +38,9 @@ __all__ = ["UnimodalDeformableDVC"]
 
 
 class UnimodalDeformableDVC(nn.Module):
+    # inference: None — the greedy decode; a dict — options of the caption decoder's ``generate``
+    caption_options = None
+
     def __init__(self, input_modalities, num_queries, d_model, num_classes, aux_loss, matcher, threshold,
                  max_eseq_length, vocab, seq_len, embedding_matrix, detr_args, caption_args,
                  use_differentiable_mask=False):
@@ -208,8 +211,8 @@ class UnimodalDeformableDVC(nn.Module):
         bos, eos, pad = special_tokens(self.vocab)
         cross = pred_memory_mask_list if self.use_differentiable_mask else memory_mask_list
         key_mask = cross[-1][:, 0, 0, :]
-        captions, last_input = self.unimodal_caption_decoder.greedy_decode(memory_list[-1], key_mask, bos, eos, pad,
-                                                                           self.seq_len - 1, faster_eval)
+        captions, last_input = decode_captions(self.unimodal_caption_decoder, (memory_list[-1], key_mask), self.vocab,
+                                               self.seq_len - 1, faster_eval, self.caption_options)
         out['pred_captions'] = self._caption_probs(last_input, memory_list[-1], cross[-1])
         captions_with_eos = append_end_token(captions, self.vocab, faster_eval)
         indices_aux = []

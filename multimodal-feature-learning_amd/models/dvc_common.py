@@ -7,7 +7,7 @@ import torch
 from ..utils.preds_postprocess import crop_segments, denormalize_segments, get_src_permutation_idx
 
 __all__ = ["special_tokens", "make_tgt_mask", "look_ahead_mask", "make_padding_mask", "segment_memory",
-           "context_mask", "append_end_token"]
+           "context_mask", "decode_captions", "append_end_token"]
 
 
 def special_tokens(vocab):
@@ -55,6 +55,21 @@ def context_mask(model, denorm, query_features_selected, key_mask):
     # seg_confidence = ones (:255-257): exactly pred (1 * p = p, (1 - 1) * m = 0, p + 0 = p) and a gradient
     # of exactly 1 — five launches each way per level that change nothing, so pred is used as it is
     return pred, pred.sigmoid() > 0.5
+
+
+def decode_captions(decoder, memories, vocab, length, faster_eval, options):
+    """The captions of an inference pass and the decoder's input at their last word (None if no word ran).
+    ``memories``: the decoder's memory and mask arguments.  ``options`` None: the reference's greedy loop; else
+    ``generate``'s (beams, penalties, a grammar)."""
+    bos, eos, pad = special_tokens(vocab)
+    if options is None:
+        return decoder.greedy_decode(*memories, bos, eos, pad, length, faster_eval)
+    captions, _ = decoder.generate(*memories, bos, eos, pad, length, **options)
+    if length < 2:
+        return captions, None
+    last_input = captions.clone()
+    last_input[:, -1] = pad
+    return captions, last_input
 
 
 def append_end_token(captions, vocab, faster_eval):

@@ -76,8 +76,11 @@ class PositionalEncoding(nn.Module):
         self.dropout = nn.Dropout(dropout)
         self.register_buffer('pos_embedding', pos_embedding.unsqueeze(0))
 
-    def forward(self, token_embedding, start=0):
-        """``start``: position of the first token (the incremental decode feeds single rows)."""
+    def forward(self, token_embedding, start=0, positions=None):
+        """``start``: position of the first token (the incremental decode feeds single rows); ``positions`` (N, L):
+        every token's own."""
+        if positions is not None:
+            return self.dropout(token_embedding + self.pos_embedding[0, positions].to(token_embedding.dtype))
         return self.dropout(token_embedding
                             + self.pos_embedding[:, start:start + token_embedding.size(1), :].to(token_embedding.dtype))
 

@@ -16,9 +16,10 @@ from .add_norm import add_layer_norm, add_layer_norm_carry, carry_supported
 from .attention import CrossAttention, masked_scores_softmax
 from .ffn import gelu_dropout
 from .linear import Linear
+from .paged_cache import PagedKVCache, paged_attention
 
 __all__ = ["MLP", "FFN", "ContextMaskModel", "UnimodalCaptionDecoderLayer", "MultimodalCaptionDecoderLayer",
-           "CaptionKVCache"]
+           "CaptionKVCache", "PagedCaptionCache"]
 
 
 class MLP(nn.Module):
@@ -89,6 +90,55 @@ class CaptionKVCache:
             self.self_k[layer_idx] = like.new_zeros(shape)
             self.self_v[layer_idx] = like.new_zeros(shape)
         return self.self_k[layer_idx], self.self_v[layer_idx]
+
+
+class PagedCaptionCache:
+    """``CaptionKVCache`` on pages (paged_cache.py) for ``generate``: rows of any number of committed words, forked and
+    freed on the device.  The pages are laid out with the first layer's keys (their type and heads); cross[layer]
+    as in ``CaptionKVCache``, one memory for all beams of a sequence."""
+
+    def __init__(self, rows, max_words, page_size, device):
+        self.rows, self.max_words, self.page_size, self.device = rows, max_words, page_size, device
+        self.kv = None
+        self.cross = {}
+        self.layers = 0
+        self._pending = None
+
+    def advance(self, parents, words, select=1):
+        """Before a chunk: row r continues row parents[r] (None: itself).  words (rows) bool: the rows that commit
+        the chunk's first row; or int32: the lengths after the chunk.  The chunk's rows are every ``select``-th row."""
+        if self.kv is None:
+            self._pending = (words, select)  # (the pages are laid out by the first attention)
+            return
+        lens = self.kv.lens if parents is None else self.kv.lens[parents]
+        self.select = select
+        self.starts = lens
+        self.kv.update(None if parents is None else parents.to(torch.int32),
+                       lens + words.to(torch.int32) if words.dtype == torch.bool else words)
+
+    def _lay_out(self, heads, head_dim, dtype):
+        self.kv = PagedKVCache(self.layers, self.rows, self.max_words, heads, head_dim, self.page_size, dtype=dtype,
+                               device=self.device)
+        words, select = self._pending
+        self.advance(None, words, select)
+
+    def self_attention(self, layer_idx, q, k, v, scale):
+        """q, k, v (n, R, H, hd) of the chunk -> heads concatenated (n, R, H * hd): row i at its sequence's i-th new
+        position, seeing the committed words up to it; its key and value are kept if the row commits it."""
+        if self.kv is None:
+            self._lay_out(k.shape[2], k.shape[3], k.dtype)
+        kv, e = self.kv, self.select
+        table, lens, starts = kv.table, kv.lens, self.starts
+        if e > 1:
+            table, lens, starts = table[::e], lens[::e], starts[::e]
+        out = paged_attention(q, kv.data[layer_idx, 0], kv.data[layer_idx, 1], table, lens, k=k, v=v, starts=starts,
+                              max_kv=self.max_words, scale=scale)
+        return out.flatten(2)
+
+
+def _rows_of(x, n):
+    """Rows (n * beams, R, d) as (n, beams * R, d): the beams of a sequence read one memory."""
+    return x if x.shape[0] == n else x.reshape(n, -1, x.shape[-1])
 
 
 def _heads(x, h):
@@ -181,6 +231,10 @@ class UnimodalCaptionDecoderLayer(nn.Module):
 
     def _sa_step(self, x, cache, layer_idx, pos):
         sa = self.self_attention
+        if isinstance(cache, PagedCaptionCache):
+            q, k, v = (f(x).unflatten(2, (sa.num_heads, -1)) for f in (sa.q_linear, sa.k_linear, sa.v_linear))
+            o = cache.self_attention(layer_idx, q, k, v, sa.scale)
+            return self.projection_dropout_1(sa.projection_layer(o))
         q, k, v = (_heads(f(x), sa.num_heads) for f in (sa.q_linear, sa.k_linear, sa.v_linear))
         o = _cached_self_attention(q, k, v, cache, layer_idx, pos, sa.scale, -1e20)
         return self.projection_dropout_1(sa.projection_layer(o.transpose(1, 2).flatten(2)))
@@ -188,12 +242,14 @@ class UnimodalCaptionDecoderLayer(nn.Module):
     def _ca_step(self, x, cache, layer_idx):
         ca = self.cross_attention
         k, v, key_mask = cache.cross[layer_idx]
-        q = _heads(ca.q_linear(x), ca.num_heads)
+        q = _heads(ca.q_linear(_rows_of(x, k.shape[0])), ca.num_heads)
         p = masked_scores_softmax(q @ k.transpose(-2, -1), key_mask, ca.scale, -1e20)
-        return self.projection_dropout_2(ca.projection_layer((p @ v).transpose(1, 2).flatten(2)))
+        o = (p @ v).transpose(1, 2).flatten(2).view(x.shape)
+        return self.projection_dropout_2(ca.projection_layer(o))
 
-    def step(self, x, cache, layer_idx, pos):
-        """x (N, R, d): row 0 committed at ``pos``, rows 1.. probes; same math as ``forward``."""
+    def step(self, x, cache, layer_idx, pos=None):
+        """x (N, R, d): row 0 committed at ``pos``, rows 1.. probes (a ``PagedCaptionCache`` knows the positions
+        and how many rows are committed); same math as ``forward``."""
         if self.pre_norm:
             x = x + self._sa_step(self.layer_norm_1(x), cache, layer_idx, pos)
             x = x + self._ca_step(self.layer_norm_2(x), cache, layer_idx)
@@ -287,9 +343,13 @@ class MultimodalCaptionDecoderLayer(nn.Module):
                          None if kpm is None else kpm[:, None, None, :])
         cache.cross[layer_idx] = ent
 
-    def step(self, x, cache, layer_idx, pos):
+    def step(self, x, cache, layer_idx, pos=None):
         def sa(h):
             mha = self.self_attention
+            if isinstance(cache, PagedCaptionCache):
+                q, k, v = (_mha_project(mha, h, i).unflatten(2, (mha.num_heads, -1)) for i in range(3))
+                o = cache.self_attention(layer_idx, q, k, v, 1.0 / math.sqrt(q.shape[-1]))
+                return self.projection_dropout_1(mha.out_proj(o))
             q, k, v = (_heads(_mha_project(mha, h, i), mha.num_heads) for i in range(3))
             o = _cached_self_attention(q, k, v, cache, layer_idx, pos, 1.0 / math.sqrt(q.shape[-1]), float("-inf"))
             return self.projection_dropout_1(mha.out_proj(o.transpose(1, 2).flatten(2)))
@@ -297,10 +357,10 @@ class MultimodalCaptionDecoderLayer(nn.Module):
         def ca(name, mha, drop):
             def f(h):
                 k, v, key_mask = cache.cross[layer_idx][name]
-                q = _heads(_mha_project(mha, h, 0), mha.num_heads)
+                q = _heads(_mha_project(mha, _rows_of(h, k.shape[0]), 0), mha.num_heads)
                 p = masked_scores_softmax(q @ k.transpose(-2, -1), key_mask, 1.0 / math.sqrt(q.shape[-1]),
                                           float("-inf"))
-                return drop(mha.out_proj((p @ v).transpose(1, 2).flatten(2)))
+                return drop(mha.out_proj((p @ v).transpose(1, 2).flatten(2).view(h.shape)))
             return f
 
         return self._combine(x, sa, ca("video", self.video_cross_attention, self.projection_dropout_2),

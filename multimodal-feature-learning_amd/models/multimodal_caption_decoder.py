@@ -10,6 +10,7 @@ dropouts, and the builder accepts either name."""
 import torch
 from torch import nn
 
+from .caption_generate import generate
 from .load_weights import init_encoder_block_weights
 from .modules.embedding_layers import PositionalEncoding, VocabularyEmbedder
 from .modules.layers import MultimodalCaptionDecoderLayer
@@ -73,6 +74,24 @@ class MultimodalCaptionDecoder(nn.Module):
 
         return greedy_decode(self, prime, step, video_memory.shape[0], length, bos, eos, pad, faster_eval,
                              video_memory.device)
+
+    def generate(self, video_memory, video_key_mask, audio_memory, audio_key_mask, bos, eos, pad, length, beams=1,
+                 **options):
+        """``UnimodalCaptionDecoder.generate`` over both memories (key masks (N, K) bool, True = masked, or None)."""
+        memories = {"video": (video_memory, video_key_mask), "audio": (audio_memory, audio_key_mask)}
+
+        def prime(cache):
+            cache.layers = len(self.decoder)
+            for i, layer in enumerate(self.decoder):
+                layer.prime(cache, i, memories)
+
+        def step(x, cache):
+            for i, layer in enumerate(self.decoder):
+                x = layer.step(x, cache, i)
+            return x
+
+        return generate(self, prime, step, video_memory.shape[0], bos, eos, pad, length, video_memory.device, beams,
+                        **options)
 
 
 def build_multimodal_caption_decoder(args, vocab_size, seq_len, embedding_matrix):

@@ -15,8 +15,8 @@ import torch
 from torch import nn
 
 from ..base_encoder import build_base_encoder
-from ..dvc_common import (append_end_token, context_mask, look_ahead_mask, make_padding_mask, segment_memory,
-                          special_tokens)
+from ..dvc_common import (append_end_token, context_mask, decode_captions, look_ahead_mask, make_padding_mask,
+                          segment_memory)
 from ..modules.embedding_layers import PositionEmbeddingVideoSine
 from ..modules.layers import FFN, ContextMaskModel
 from ..modules.linear import Linear
@@ -43,6 +43,9 @@ def decoder_reference_stack(init_reference, inter_references):
 
 
 class UnimodalSparseDVC(nn.Module):
+    # inference: None — the greedy decode; a dict — options of the caption decoder's ``generate``
+    caption_options = None
+
     def __init__(self, input_modalities, num_queries, d_model, num_classes, aux_loss, matcher, threshold,
                  max_eseq_length, vocab, seq_len, embedding_matrix, sparse_detr_args, caption_args,
                  use_differentiable_mask=False):
@@ -154,9 +157,8 @@ class UnimodalSparseDVC(nn.Module):
             out["pred_captions"] = outputs_caption[-1]
             captions_out = torch.argmax(outputs_caption[-1], dim=2)
         elif val_mode == "one_by_one":
-            bos, eos, pad = special_tokens(self.vocab)
-            captions, last_input = self.unimodal_caption_decoder.greedy_decode(memory, key_mask, bos, eos, pad,
-                                                                               self.seq_len, faster_eval)
+            captions, last_input = decode_captions(self.unimodal_caption_decoder, (memory, key_mask), self.vocab,
+                                                   self.seq_len, faster_eval, self.caption_options)
             outputs_caption = self._caption_probs(last_input, memory, key_mask)
             out['pred_captions'] = outputs_caption[-1]
             captions_out = append_end_token(captions, self.vocab, faster_eval)

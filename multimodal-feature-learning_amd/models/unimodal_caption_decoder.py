@@ -11,6 +11,7 @@ import torch
 from torch import nn
 
 from .. import _trace
+from .caption_generate import generate
 from .load_weights import init_encoder_block_weights
 from .modules.embedding_layers import PositionalEncoding, VocabularyEmbedder
 from .modules.layers import CaptionKVCache, UnimodalCaptionDecoderLayer
@@ -169,6 +170,30 @@ class UnimodalCaptionDecoder(nn.Module):
             return x
 
         return greedy_decode(self, prime, step, memory.shape[0], length, bos, eos, pad, faster_eval, memory.device)
+
+    def generate(self, memory, memory_key_mask, bos, eos, pad, length, beams=1, **options):
+        """Captions by beam search from a paged cache: (captions (N, ``length``) int32, scores (N) float32, the sum of
+        the words' log-probabilities).  memory (N, K, d), memory_key_mask (N, K) bool (True = masked) or None.
+        ``beams`` captions a sequence; ``prompt`` (N, words) int words that every caption begins with after <bos>
+        (prompt_lens (N): how many of them; no <pad> among them); ``repetition``, ``presence``, ``frequency``, ``bias``: of
+        ``process_logits`` (modules/logits.py), over the words so far, <bos> excepted (those of single rows need
+        beams = 1).  ``allowed`` (vocab) bool, or a
+        grammar: (states, vocab) bool with ``transitions`` (states, vocab), the state after each word, from
+        state 0.  Scores are divided by the number of words ** ``length_penalty`` before the best beam is taken.
+        A caption is <bos>, its words, <eos>, then <pad>.  With one beam and no options: greedy_decode's words."""
+        mask4 = None if memory_key_mask is None else memory_key_mask[:, None, None, :]
+
+        def prime(cache):
+            cache.layers = len(self.decoder)
+            for i, layer in enumerate(self.decoder):
+                layer.prime(cache, i, memory, mask4)
+
+        def step(x, cache):
+            for i, layer in enumerate(self.decoder):
+                x = layer.step(x, cache, i)
+            return x
+
+        return generate(self, prime, step, memory.shape[0], bos, eos, pad, length, memory.device, beams, **options)
 
 
 def build_unimodal_caption_decoder(args, vocab_size, seq_len, embedding_matrix):
