@@ -11,10 +11,17 @@
 // values' 16-bit type for the matrix product (relative 2^-9 / 2^-12 of each weight, against the output's
 // own rounding of the same size); l sums the unrounded weights.
 //
+// The reference value m follows the maximum only when that has grown by more than 2^8 (any m gives the same
+// quotient): most steps then need no rescale of O and no exchange between lanes.
+//
 //   paged_att_split  few rows a (sequence, key head): a workgroup takes 32 rows and a range of the keys,
-//                    its waves equal parts of the range; the waves' (m, l, O) meet in LDS, the ranges' in
-//   paged_att_join   the workspace.
-//   paged_att_rows   many rows: 4 waves of 32 rows share 64-key tiles in LDS.
+//                    its two waves halves of it, each through its own ring of tiles in LDS; their (m, l, O) meet in LDS
+//   paged_att_rows   many rows: 4 waves of 32 rows share double-buffered tiles of 64 keys
+//   paged_att_join   key ranges of either: (m, l, O) of a row out of the workspace
+//
+// Keys and values go to LDS by global_load_lds (16 bytes a lane): no registers are held while the loads fly,
+// so a wave keeps 16 to 32 KB in flight.  Rows of one load lie in one page where the page holds as many
+// (4 rows at 256 bytes): its address is then scalar and the lane's offset constant.
 //
 // MFMA 32x32x16 (16-bit): A lane (h, r): row r = lane & 31, k 8h..8h+7 (h = lane >> 5); B the same with
 // columns; D register e: row 8 (e >> 2) + 4 h + (e & 3), column lane & 31.  The reduction of the second
@@ -50,7 +57,8 @@ struct Args {
   float* ws;
   const int *table, *kv_lens, *starts, *offsets;
   int n, rows, heads, kvh, G, D, pages, ps, sh, width, causal, splits, tiles, zero_tail;
-  long long total;
+  int range;              // keys a split takes at least
+  long long total, slots; // packed rows; rows of the whole call (of a partial in the workspace)
   long long q_seq, q_row, q_head, k_seq, k_row, k_head, v_seq, v_row, v_head;  // bytes
   float c;  // scale * log2(e)
 };
@@ -95,19 +103,20 @@ struct Geo {
 
 struct Seq {
   int st, kv, rows;      // first position, visible length, rows of this call
-  long long q0;          // packed: first row; else 0 (the sequence stride is in the base pointers)
+  long long q0, q1;      // packed: first row and the one behind the last; else 0 (the strides are in the pointers)
 };
 
 __device__ __forceinline__ Seq seq_of(const Args& a, int s) {
   Seq q;
   q.kv = max(0, min(a.kv_lens[s], a.width * a.ps));  // (width * page_size < 2^31: checked on the host)
-  q.q0 = 0;
+  q.q0 = q.q1 = 0;
   q.rows = a.rows;
   int len = a.rows;
   if (a.offsets) {
     const long long o0 = max(0ll, min((long long)a.offsets[s], a.total));
     const long long o1 = max(o0, min((long long)a.offsets[s + 1], a.total));
     q.q0 = o0;
+    q.q1 = o1;
     len = (int)(o1 - o0);
     q.rows = min(len, a.rows);
   }
@@ -137,12 +146,111 @@ __device__ __forceinline__ bool row_src(const Args& a, const Seq& q, const unsig
   return true;
 }
 
+// 16 bytes a lane from global memory to LDS at byte `dst` + 16 * lane (dst: wave-uniform, below 64 KB).
+// The loads count in vmcnt; nothing but wait_loads() waits for them
+__device__ __forceinline__ void load_lds(const unsigned char* base, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void load_lds(const unsigned char* src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst)
+               : "memory", "m0");
+}
+// all but the last N vector memory operations of the wave are done
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "vmcnt has six bits");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// a barrier that does not wait for loads to LDS, and that no LDS access crosses
+__device__ __forceinline__ void wave_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+
+// 64 entries of a sequence's table a time, one a lane, and the next 64 on their way
+struct Pages {
+  int base, cur, nxt;
+  unsigned long long bad;  // entries of `cur` outside the pool
+
+  __device__ __forceinline__ int entry(const Args& a, const int* tab, int i) const { return i < a.width ? tab[i] : -1; }
+  __device__ __forceinline__ void start(const Args& a, const int* tab, int first, int lane) {
+    base = first;
+    cur = entry(a, tab, base + lane);
+    nxt = entry(a, tab, base + 64 + lane);
+    bad = __ballot((unsigned)cur >= (unsigned)a.pages);
+  }
+  // entries first .. last (uniform, ascending from call to call, fewer than 64 of them from a multiple) are in `cur`
+  __device__ __forceinline__ void need(const Args& a, const int* tab, int first, int last, int lane) {
+    if (last - base < 64) return;
+    if (first - base == 64) {
+      base += 64;
+      cur = nxt;
+      nxt = entry(a, tab, base + 64 + lane);
+      bad = __ballot((unsigned)cur >= (unsigned)a.pages);
+    } else {
+      start(a, tab, first, lane);
+    }
+  }
+  __device__ __forceinline__ bool any_bad(int first, int last) const {
+    const int w = last - first + 1;
+    return ((bad >> (first - base)) & (w >= 64 ? ~0ull : (1ull << w) - 1ull)) != 0ull;
+  }
+};
+
+// loads of 1 KB (64 lanes) for image rows r0 .. of keys j0 + r0 ..: IT of them for keys and values each, LDS images
+// at kd and vd.  `safe`: keys below it come from the pages and are there
+template <class T, int DP, int IT>
+__device__ __forceinline__ void load_tile(const Args& a, const Seq& q, const Pages& pg, const unsigned char* kn,
+                                          const unsigned char* vn, int kh, int j0, int r0, int safe, uint32_t kd,
+                                          uint32_t vd, int lane) {
+  typedef Geo<T, DP> Ge;
+  constexpr int RP = 64 / Ge::NC;  // rows a load
+  const int rb = a.D * Ge::EB, nch = rb / 16;
+  const int lr = lane / Ge::NC, cp = lane % Ge::NC;
+  const int jb = j0 + r0;
+  const int e0 = jb >> a.sh, e1 = (jb + IT * RP - 1) >> a.sh;
+  if (jb + IT * RP <= safe && a.ps >= RP && !pg.any_bad(e0, e1)) {
+#pragma unroll
+    for (int t = 0; t < IT; ++t) {
+      const int row = r0 + t * RP + lr;
+      const int j = jb + t * RP;
+      const int page = __builtin_amdgcn_readlane(pg.cur, (j >> a.sh) - pg.base);
+      const long long off = (((long long)page * a.kvh + kh) * a.ps + (j & (a.ps - 1))) * rb;
+      const int ck = cp ^ Ge::k_swz(row), cv = cp ^ Ge::v_swz(row);
+      if (ck < nch) load_lds(a.kp + off, (uint32_t)(lr * rb + ck * 16), kd + (r0 / RP + t) * 1024);
+      if (cv < nch) load_lds(a.vp + off, (uint32_t)(lr * rb + cv * 16), vd + (r0 / RP + t) * 1024);
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < IT; ++t) {
+      const int row = r0 + t * RP + lr;
+      const int j = j0 + row;
+      const int page = __shfl(pg.cur, (j >> a.sh) - pg.base);
+      RowSrc r;
+      row_src(a, q, kn, vn, kh, j, page, rb, r);
+      const int ck = cp ^ Ge::k_swz(row), cv = cp ^ Ge::v_swz(row);
+      if (ck < nch) load_lds(r.k + ck * 16, kd + (r0 / RP + t) * 1024);
+      if (cv < nch) load_lds(r.v + cv * 16, vd + (r0 / RP + t) * 1024);
+    }
+  }
+}
+
+// chunks behind a row's D elements: zero once, the loads leave them alone
+template <class T, int DP>
+__device__ __forceinline__ void clear_lds(unsigned char* lds, int bytes, int tid, int threads) {
+  for (int i = tid * 16; i < bytes; i += threads * 16) *reinterpret_cast<uint4*>(lds + i) = uint4{0, 0, 0, 0};
+}
+
 // the rows of a wave, as MFMA columns
 template <class T, int DP>
 struct Cols {
   uint4 qf[Geo<T, DP>::QF];
   f32x16 o[Geo<T, DP>::OB];
-  float m, l;
+  float m, l;  // reference value; sum of the weights (of the lane's own scores until cols_sum)
   int lim;  // keys this lane's row sees
 };
 
@@ -264,6 +372,29 @@ __device__ __forceinline__ bool scrub(uint4& v) {
   return any;
 }
 
+// the same over an LDS image (its loads have been waited for); the wave's later reads see the result
+template <class T>
+__device__ __forceinline__ bool scrub_image(unsigned char* p, int bytes, int lane, int lanes) {
+  bool any = false;
+#pragma unroll 1
+  for (int i = lane * 16; i < bytes; i += lanes * 16) {
+    uint4 v = *reinterpret_cast<const uint4*>(p + i);
+    if (scrub<T>(v)) {
+      *reinterpret_cast<uint4*>(p + i) = v;
+      any = true;
+    }
+  }
+  wait_lds();
+  return any;
+}
+
+// bit kk: key j0 + kk lies in a page of the pool (asked only where a tile has one that does not)
+__device__ __forceinline__ uint32_t keys_there(const Args& a, const int* tab, int j0, int kv, int lane) {
+  const int j = j0 + (lane & 31);
+  const int page = j < kv ? tab[j >> a.sh] : -1;
+  return (uint32_t)__ballot((unsigned)page < (unsigned)a.pages);
+}
+
 // scores of keys j0 .. j0+31 that the lane's row does not see become -inf; `there` bit kk: key j0+kk exists
 __device__ __forceinline__ void mask_scores(f32x16& s, int j0, int lim, uint32_t there, int lane) {
   const int h = lane >> 5;
@@ -274,7 +405,9 @@ __device__ __forceinline__ void mask_scores(f32x16& s, int j0, int lim, uint32_t
   }
 }
 
-// the online softmax's step for NT score tiles: m, l and O rescaled, s replaced by the weights
+// the online softmax's step for NT score tiles: s replaced by the weights against m; m, l and O rescaled when
+// some row's maximum outgrows m by 2^kLazy.  w.l: the sum of the lane's own scores only
+constexpr float kLazy = 8.f;
 template <class T, int DP, int NT>
 __device__ __forceinline__ void soft_step(Cols<T, DP>& w, f32x16 (&s)[NT], float c) {
   float mx = s[0][0];
@@ -282,25 +415,27 @@ __device__ __forceinline__ void soft_step(Cols<T, DP>& w, f32x16 (&s)[NT], float
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
-  mx = fmaxf(mx, __shfl_xor(mx, 32));
-  const float mn = fmaxf(w.m, mx);
-  const float base = mn == -INFINITY ? 0.f : mn * c;  // (nothing seen yet: every weight is 2^-inf = 0)
-  const float al = __builtin_amdgcn_exp2f(fmaf(w.m, c, -base));
-  float sum = 0.f;
+  if (__any((mx - w.m) * c > kLazy)) {  // (-inf - -inf: false, nothing seen yet)
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float mn = fmaxf(w.m, mx);
+    const float al = __builtin_amdgcn_exp2f(w.m == mn ? 0.f : (w.m - mn) * c);
+    w.m = mn;
+    w.l *= al;
+#pragma unroll
+    for (int d = 0; d < Geo<T, DP>::OB; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w.o[d][e] *= al;
+  }
+  const float base = w.m == -INFINITY ? 0.f : w.m * c;  // (nothing seen yet: every weight is 2^-inf = 0)
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, -base));
-      sum += s[t][e];
+      sum[e & 3] += s[t][e];
     }
-  sum += __shfl_xor(sum, 32);
-  w.l = w.l * al + sum;
-  w.m = mn;
-#pragma unroll
-  for (int d = 0; d < Geo<T, DP>::OB; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) w.o[d][e] *= al;
+  w.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 template <class T>
@@ -384,108 +519,209 @@ __device__ __forceinline__ void write_chunk(const Args& a, const Seq& q, int s, 
   }
 }
 
-// packed rows behind the last sequence's
-__device__ __forceinline__ void zero_rows(const Args& a, int part, int parts, int eb) {
-  const long long r0 = max(0ll, min((long long)a.offsets[a.n], a.total));
+// packed rows first .. last - 1 of `out`
+__device__ __forceinline__ void zero_rows(const Args& a, long long first, long long last, int part, int parts, int eb) {
   const long long per = (long long)a.heads * a.D * eb / 16;
-  uint4* dst = reinterpret_cast<uint4*>(a.out) + r0 * per;
-  for (long long e = (long long)part * blockDim.x + threadIdx.x; e < (a.total - r0) * per;
+  uint4* dst = reinterpret_cast<uint4*>(a.out);
+  for (long long e = first * per + (long long)part * blockDim.x + threadIdx.x; e < last * per;
        e += (long long)parts * blockDim.x)
     dst[e] = uint4{0, 0, 0, 0};
 }
 
-// grid: x = splits * tiles (tile major), y = kv heads, z folded into x through n (x = ((s * tiles) + tile) *
-// splits + split; s == n: the rows behind the last sequence)
+template <class T, int DP>
+__device__ __forceinline__ void cols_sum(Cols<T, DP>& w) {
+  w.l += __shfl_xor(w.l, 32);
+}
+
+// What the ranges of a row leave in the workspace: `used` (slots * heads int32: how many ranges, 0 or 1: nothing to
+// join), then per range (m, l) pairs and O rows of DP floats, slots * heads of each
+struct Part {
+  int* used;
+  float *ml, *o;
+};
+__device__ __forceinline__ Part part_of(const Args& a, int split, int DP) {
+  const long long sh = a.slots * a.heads;
+  Part p;
+  p.used = reinterpret_cast<int*>(a.ws);
+  float* f = a.ws + (sh + 3) / 4 * 4;
+  p.ml = f + split * sh * 2;
+  p.o = f + (a.splits * sh * 2 + 3) / 4 * 4 + split * sh * DP;
+  return p;
+}
+
+template <class T, int DP>
+__device__ __forceinline__ void cols_part(const Cols<T, DP>& w, const Args& a, const Seq& q, int s, int kh, int m0,
+                                          int split, int used, int lane) {
+  const int row = m0 + (lane & 31), h = lane >> 5;
+  const int i = row / a.G, g = row - i * a.G;
+  if (i >= q.rows) return;
+  const Part p = part_of(a, split, DP);
+  const long long id = ((a.offsets ? q.q0 : (long long)s * a.rows) + i) * a.heads + kh * a.G + g;
+  if (h == 0) {
+    if (split == 0) p.used[id] = used;
+    p.ml[id * 2] = w.m;
+    p.ml[id * 2 + 1] = w.l;
+  }
+#pragma unroll
+  for (int d = 0; d < Geo<T, DP>::OB; ++d)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int col = d * 32 + 8 * b + 4 * h;
+      if (col < a.D)
+        *reinterpret_cast<f32x4*>(p.o + id * DP + col) =
+            f32x4{w.o[d][4 * b], w.o[d][4 * b + 1], w.o[d][4 * b + 2], w.o[d][4 * b + 3]};
+    }
+}
+
+// a row written whole: nothing for the join to do
+__device__ __forceinline__ void mark_whole(const Args& a, const Seq& q, int s, int kh, int m0, int lane) {
+  const int row = m0 + (lane & 31);
+  const int i = row / a.G, g = row - i * a.G;
+  if (i >= q.rows || lane >= 32) return;
+  reinterpret_cast<int*>(a.ws)[((a.offsets ? q.q0 : (long long)s * a.rows) + i) * a.heads + kh * a.G + g] = 1;
+}
+
+// packed rows first .. last - 1 are not this call's to write
+__device__ __forceinline__ void mark_rows(const Args& a, long long first, long long last, int part, int parts) {
+  for (long long e = first * a.heads + (long long)part * blockDim.x + threadIdx.x; e < last * a.heads;
+       e += (long long)parts * blockDim.x)
+    reinterpret_cast<int*>(a.ws)[e] = 0;
+}
+
+// what a workgroup has to do, the same in both kernels.  Work items are numbered ((s * tiles + tile) * splits +
+// split) * kvh + kh: the workgroups that read one key head's pages are kvh apart and, with 8 XCDs taking
+// workgroups in turn, share an L2 when kvh is a multiple of 8 (and a half or a quarter of them when it is 4 or 2)
+struct Job {
+  int s, tile, split, kh;
+};
+__device__ __forceinline__ Job job_of(const Args& a) {
+  Job j;
+  unsigned x = blockIdx.x;
+  j.kh = x % (unsigned)a.kvh;
+  x /= (unsigned)a.kvh;
+  j.split = x % (unsigned)a.splits;
+  x /= (unsigned)a.splits;
+  j.tile = a.tiles - 1 - x % (unsigned)a.tiles;  // (a sequence's last rows see the most keys: they begin first)
+  j.s = x / (unsigned)a.tiles;
+  return j;
+}
+
+// packed calls (s == n): the rows before the first sequence and behind the last
+__device__ __forceinline__ void rest_of_rows(const Args& a, const Job& j, int eb) {
+  const int part = (j.tile * a.splits + j.split) * a.kvh + j.kh, parts = a.tiles * a.splits * a.kvh;
+  const long long r0 = max(0ll, min((long long)a.offsets[0], a.total));
+  const long long r1 = max(r0, min((long long)a.offsets[a.n], a.total));
+  if (a.zero_tail) {
+    zero_rows(a, 0, r0, part, parts, eb);
+    zero_rows(a, r1, a.total, part, parts, eb);
+  }
+  if (a.splits > 1) {
+    mark_rows(a, 0, r0, part, parts);
+    mark_rows(a, r1, a.total, part, parts);
+  }
+}
+// ... and a sequence's rows behind its first a.rows
+__device__ __forceinline__ void rows_behind(const Args& a, const Job& j, const Seq& q) {
+  if (a.splits > 1 && a.offsets && q.q1 > q.q0 + q.rows)
+    mark_rows(a, q.q0 + q.rows, q.q1, (j.tile * a.splits + j.split) * a.kvh + j.kh, a.tiles * a.splits * a.kvh);
+}
+
+// keys first .. last - 1 (multiples of `step` but the last) of `most` that range `split` takes; used: ranges in all
+struct Range {
+  int first, last, used;
+};
+__device__ __forceinline__ Range range_of(const Args& a, int most, int split, int step) {
+  const int steps = (most + step - 1) / step;
+  const int per = max(a.range / step, (steps + a.splits - 1) / a.splits);
+  Range r;
+  r.used = max(1, (steps + per - 1) / per);
+  r.first = min(most, split * per * step);
+  r.last = min(most, r.first + per * step);
+  return r;
+}
+
 template <class T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) void paged_att_split(Args a) {
+__global__ __launch_bounds__(64 * NW, 1) void paged_att_split(Args a) {
   typedef Geo<T, DP> Ge;
-  constexpr int kImg = kKeys * Ge::RB;                       // one 32-row image
+  constexpr int kImg = kKeys * Ge::RB;  // one 32-row image
+  constexpr int kStage = 2 * kImg;      // keys and values
+  constexpr int NS = kStage >= 32768 ? 1 : kStage >= 16384 ? 2 : 4;  // stages of a wave's ring (at most 32 KB)
+  constexpr int kIt = kImg / 1024;      // loads of one image
   constexpr int kMerge = NW > 1 ? NW * 32 * (DP + 1) * 4 : 0;
-  constexpr int kLds = NW * 2 * kImg > kMerge ? NW * 2 * kImg : kMerge;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[kLds];
+  constexpr int kLds = NW * NS * kStage > kMerge ? NW * NS * kStage : kMerge;
+  static_assert(NW * NS * kStage <= 65536, "load_lds reaches 64 KB");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[kLds];
   __shared__ float s_m[NW][32], s_l[NW][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  int x = blockIdx.x;
-  const int split = x % a.splits;
-  x /= a.splits;
-  const int tile = x % a.tiles, s = x / a.tiles, kh = blockIdx.y;
+  const Job job = job_of(a);
+  const int s = job.s, kh = job.kh, split = job.split;
   if (s >= a.n) {
-    zero_rows(a, (tile * a.splits + split) * a.kvh + kh, a.tiles * a.splits * a.kvh, Ge::EB);
+    rest_of_rows(a, job, Ge::EB);
     return;
   }
   const Seq q = seq_of(a, s);
-  const int m0 = tile * kRowsW;
-  if (m0 >= q.rows * a.G) return;  // (uniform over the workgroup; the join skips these tiles the same way)
+  rows_behind(a, job, q);
+  const int m0 = job.tile * kRowsW;
+  if (m0 >= q.rows * a.G) return;  // (uniform over the workgroup)
+  const int ilast = min(q.rows - 1, (m0 + kRowsW - 1) / a.G);
+  const int most = a.causal ? max(0, min(q.kv, q.st + ilast + 1)) : q.kv;  // keys the tile's last row sees
+  const Range rg = range_of(a, most, split, kKeys);
+  if (split >= rg.used) return;
   const long long seq = a.offsets ? 0 : s;
   const unsigned char* qb = a.q + seq * a.q_seq + q.q0 * a.q_row;
   const unsigned char* kn = a.kn ? a.kn + seq * a.k_seq + q.q0 * a.k_row + (long long)kh * a.k_head : nullptr;
   const unsigned char* vn = a.vn ? a.vn + seq * a.v_seq + q.q0 * a.v_row + (long long)kh * a.v_head : nullptr;
+  const int* tab = a.table + (long long)s * a.width;
+  const int b0 = rg.first / kKeys, b1 = (rg.last + kKeys - 1) / kKeys;
+  const int wper = (b1 - b0 + NW - 1) / NW;
+  const int w0 = b0 + wave * wper, w1 = min(b1, w0 + wper);
+  unsigned char* ring = lds + wave * NS * kStage;
+  const uint32_t ring_at = __builtin_amdgcn_readfirstlane(lds_at(ring));
+  if (a.D != DP) {
+    clear_lds<T, DP>(ring, NS * kStage, lane, 64);
+    wait_lds();
+  }
+  const int safe = a.kn ? max(0, min(q.kv, q.st)) : q.kv;
+  Pages pg;
+  uint32_t gaps = 0;  // bit of a stage: a page of its keys is outside the pool
+  if (w0 < w1) pg.start(a, tab, (w0 * kKeys) >> a.sh, lane);
+  const auto issue = [&](int blk) {
+    const int j0 = blk * kKeys;
+    pg.need(a, tab, j0 >> a.sh, (j0 + kKeys - 1) >> a.sh, lane);
+    const uint32_t slot = (uint32_t)(blk - w0) % NS, at = ring_at + slot * kStage;
+    const bool gap = pg.any_bad(j0 >> a.sh, (min(q.kv, j0 + kKeys) - 1) >> a.sh);
+    gaps = (gaps & ~(1u << slot)) | ((uint32_t)gap << slot);
+    load_tile<T, DP, kIt>(a, q, pg, kn, vn, kh, j0, 0, safe, at, at + kImg, lane);
+  };
+#pragma unroll
+  for (int t = 0; t < NS; ++t)
+    if (w0 + t < w1) issue(w0 + t);
   Cols<T, DP> w;
   cols_init<T, DP>(w, a, q, qb, kh, m0, lane);
-  // the last row of the tile sees the most keys
-  const int ilast = min(q.rows - 1, (m0 + kRowsW - 1) / a.G);
-  const int most = a.causal ? max(0, min(q.kv, q.st + ilast + 1)) : q.kv;
-  const int nblk = (most + kKeys - 1) / kKeys;
-  const int per = (nblk + a.splits - 1) / a.splits;
-  const int b0 = split * per, b1 = min(nblk, b0 + per);
-  const int wper = (max(0, b1 - b0) + NW - 1) / NW;
-  const int w0 = b0 + wave * wper, w1 = min(b1, w0 + wper);
-  unsigned char* kt = lds + wave * 2 * kImg;
-  unsigned char* vt = kt + kImg;
-  const int* tab = a.table + (long long)s * a.width;
-  const int rb = a.D * Ge::EB, nch = rb / 16;
-  constexpr int kIt = kImg / 1024;  // 16-byte loads a lane for one image
-  int pbase = 0, pg = 0;
-  uint4 rk[kIt], rv[kIt];
-  uint32_t there = 0;
   bool odd = false;  // a value that is not finite was scrubbed
   const int least = a.causal ? max(0, min(q.kv, q.st + m0 / a.G + 1)) : q.kv;  // keys the tile's first row sees
-  const auto fetch = [&](int blk) {
-    const int j0 = blk * kKeys;
-    const int pi0 = j0 >> a.sh;
-    if (blk == w0 || pi0 - pbase + ((kKeys - 1) >> a.sh) >= 64) {  // the table's next 64 entries, one a lane
-      pbase = pi0;
-      const int e = pbase + lane;
-      pg = e < a.width ? tab[e] : -1;
-    }
-#pragma unroll
-    for (int t = 0; t < kIt; ++t) {
-      const int ci = t * 64 + lane, row = ci / Ge::NC, cp = ci % Ge::NC;
-      const int j = j0 + row;
-      const int page = __shfl(pg, (j >> a.sh) - pbase);
-      RowSrc r;
-      row_src(a, q, kn, vn, kh, j, page, rb, r);
-      const int ck = cp ^ Ge::k_swz(row), cv = cp ^ Ge::v_swz(row);
-      rk[t] = ck < nch ? *reinterpret_cast<const uint4*>(r.k + ck * 16) : uint4{0, 0, 0, 0};
-      rv[t] = cv < nch ? *reinterpret_cast<const uint4*>(r.v + cv * 16) : uint4{0, 0, 0, 0};
-    }
-    const int j = j0 + (lane & 31);
-    const int page = __shfl(pg, (j >> a.sh) - pbase);
-    there = (uint32_t)__ballot(j < q.kv && (unsigned)page < (unsigned)a.pages);
-  };
-  if (w0 < w1) fetch(w0);
   for (int blk = w0; blk < w1; ++blk) {
-    if (least < min(q.kv, (blk + 1) * kKeys)) {
-#pragma unroll
-      for (int t = 0; t < kIt; ++t) odd |= scrub<T>(rv[t]);
-    }
-#pragma unroll
-    for (int t = 0; t < kIt; ++t) {
-      *reinterpret_cast<uint4*>(kt + (t * 64 + lane) * 16) = rk[t];
-      *reinterpret_cast<uint4*>(vt + (t * 64 + lane) * 16) = rv[t];
-    }
-    const uint32_t now = there;
-    if (blk + 1 < w1) fetch(blk + 1);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the wave's own LDS writes; no other wave reads them)
+    unsigned char* kt = ring + (uint32_t)(blk - w0) % NS * kStage;
+    unsigned char* vt = kt + kImg;
+    const int j0 = blk * kKeys;
+    if (blk + NS <= w1)
+      wait_loads<(NS - 1) * 2 * kIt>();
+    else
+      wait_loads<0>();
+    if (least < min(q.kv, j0 + kKeys)) odd |= scrub_image<T>(vt, kImg, lane, 64);
     f32x16 sc[1];
     sc[0] = scores<T, DP>(w, kt, lane);
-    const bool full = now == 0xffffffffu && __all((blk + 1) * kKeys <= w.lim);
-    if (!full) mask_scores(sc[0], blk * kKeys, w.lim, now, lane);
+    const bool gap = (gaps >> ((uint32_t)(blk - w0) % NS)) & 1u;
+    if (gap || !__all(j0 + kKeys <= w.lim))
+      mask_scores(sc[0], j0, w.lim, gap ? keys_there(a, tab, j0, q.kv, lane) : ~0u, lane);
     soft_step<T, DP, 1>(w, sc, a.c);
     weigh<T, DP>(w, sc[0], vt, lane);
+    wait_lds();  // (the images are read: the next loads may overwrite them)
+    if (blk + NS < w1) issue(blk + NS);
   }
   if (__any(odd))
     add_non_finite<T, DP>(w, a, q, kn, vn, tab, kh, max(w0, least / kKeys) * kKeys, min(most, w1 * kKeys), lane);
+  cols_sum<T, DP>(w);
   if (a.kn && split == 0) {
     // the tile writes the tokens whose first row it holds
     const int i0 = (m0 + a.G - 1) / a.G, i1 = min(q.rows, (m0 + kRowsW + a.G - 1) / a.G);
@@ -527,169 +763,177 @@ __global__ __launch_bounds__(64 * NW) void paged_att_split(Args a) {
         w.o[d][e] = t;
       }
   }
-  if (a.splits == 1) {
+  if (rg.used > 1) {
+    cols_part<T, DP>(w, a, q, s, kh, m0, split, rg.used, lane);
+  } else {
     cols_store<T, DP>(w, a, q, s, kh, m0, lane);
-    return;
+    if (a.splits > 1) mark_whole(a, q, s, kh, m0, lane);
   }
-  // partial: per (s, kh, tile, split): 32 maxima, 32 sums, then 32 rows of DP
-  const long long id = (((long long)s * a.kvh + kh) * a.tiles + tile) * a.splits + split;
-  float* ws = a.ws + id * (64 + 32 * DP);
-  const int col = lane & 31, h = lane >> 5;
-  if (h == 0) {
-    ws[col] = w.m;
-    ws[32 + col] = w.l;
-  }
-#pragma unroll
-  for (int d = 0; d < Ge::OB; ++d)
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-      *reinterpret_cast<f32x4*>(ws + 64 + col * DP + d * 32 + 8 * b + 4 * h) =
-          f32x4{w.o[d][4 * b], w.o[d][4 * b + 1], w.o[d][4 * b + 2], w.o[d][4 * b + 3]};
 }
 
-// one workgroup a (sequence, key head, tile): out = sum_i 2^(c (m_i - m)) O_i / sum_i 2^(c (m_i - m)) l_i
-template <class T, int DP>
+// out = sum_i 2^(c (m_i - m)) O_i / sum_i 2^(c (m_i - m)) l_i over a row's ranges.  DP / 4 lanes hold a row's
+// columns; a workgroup takes 256 / (DP / 4) rows, or (WIDE: many ranges) one row whose ranges its groups share
+template <class T, int DP, bool WIDE>
 __global__ __launch_bounds__(256) void paged_att_join(Args a) {
-  const int tile = blockIdx.x % a.tiles, s = blockIdx.x / a.tiles, kh = blockIdx.y;
-  const Seq q = seq_of(a, s);
-  const int m0 = tile * kRowsW;
-  const int nrow = min(kRowsW, q.rows * a.G - m0);
-  if (nrow <= 0) return;
-  const long long id = (((long long)s * a.kvh + kh) * a.tiles + tile) * a.splits;
-  const float* ws = a.ws + id * (64 + 32 * DP);
-  constexpr int kQ = DP / 4;  // quads a row
-  for (int e = threadIdx.x; e < nrow * kQ; e += 256) {
-    const int r = e / kQ, col = (e % kQ) * 4;
-    if (col >= a.D) continue;
-    float mx = -INFINITY;
-    for (int i = 0; i < a.splits; ++i) mx = fmaxf(mx, ws[(long long)i * (64 + 32 * DP) + r]);
-    const float base = mx == -INFINITY ? 0.f : mx * a.c;
-    float l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < a.splits; ++i) {
-      const float* p = ws + (long long)i * (64 + 32 * DP);
-      const float f = __builtin_amdgcn_exp2f(fmaf(p[r], a.c, -base));
-      l += p[32 + r] * f;
-      const f32x4 v = *reinterpret_cast<const f32x4*>(p + 64 + r * DP + col);
+  constexpr int kQ = DP / 4, kGr = 256 / kQ;
+  __shared__ float s_m[kGr], s_l[kGr];
+  __shared__ __attribute__((aligned(16))) float s_o[WIDE ? kGr : 1][DP];
+  const int gr = threadIdx.x / kQ, col = threadIdx.x % kQ * 4;
+  const long long sh = a.slots * a.heads;
+  const long long id = WIDE ? (long long)blockIdx.x : (long long)blockIdx.x * kGr + gr;
+  const Part p = part_of(a, 0, DP);
+  const int used = id < sh ? min(p.used[id], a.splits) : 0;  // (offsets that do not ascend leave rows unmarked)
+  if (WIDE && used <= 1) return;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (used > 1) {
+    const int i0 = WIDE ? gr : 0;
+    constexpr int kStep = WIDE ? kGr : 1;
+#pragma unroll 4
+    for (int i = i0; i < used; i += kStep) {
+      const float mi = p.ml[(i * sh + id) * 2], li = p.ml[(i * sh + id) * 2 + 1];
+      const f32x4 v = *reinterpret_cast<const f32x4*>(p.o + (i * sh + id) * DP + col);  // (behind D: not used)
+      const float mn = fmaxf(m, mi), base = mn == -INFINITY ? 0.f : mn * a.c;
+      const float f0 = __builtin_amdgcn_exp2f(fmaf(m, a.c, -base)), f1 = __builtin_amdgcn_exp2f(fmaf(mi, a.c, -base));
+      m = mn;
+      l = l * f0 + li * f1;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] += v[k] * f;
+      for (int k = 0; k < 4; ++k) o[k] = o[k] * f0 + v[k] * f1;
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    const int row = m0 + r, i = row / a.G, g = row - i * a.G;
-    const long long rr = (a.offsets ? q.q0 : (long long)s * a.rows) + i;
-    float v[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = o[k] * inv;
-    store4<T>(a.out + ((rr * a.heads + kh * a.G + g) * (long long)a.D + col) * (long long)sizeof(T), v);
   }
+  if constexpr (WIDE) {
+    if (col == 0) {
+      s_m[gr] = m;
+      s_l[gr] = l;
+    }
+    *reinterpret_cast<f32x4*>(&s_o[gr][col]) = o;
+    __syncthreads();
+    if (gr != 0) return;
+    float mx = -INFINITY;
+    for (int i = 0; i < kGr; ++i) mx = fmaxf(mx, s_m[i]);
+    const float base = mx == -INFINITY ? 0.f : mx * a.c;
+    l = 0.f;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < kGr; ++i) {
+      const float f = __builtin_amdgcn_exp2f(fmaf(s_m[i], a.c, -base));
+      l += s_l[i] * f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] += s_o[i][col + k] * f;
+    }
+  }
+  if (used <= 1 || col >= a.D) return;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  float v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = o[k] * inv;
+  store4<T>(a.out + (id * (long long)a.D + col) * (long long)sizeof(T), v);
 }
 
 constexpr int kWavesR = 4;
 constexpr int kTileR = kWavesR * kRowsW;  // rows a workgroup of paged_att_rows
 
 template <class T, int DP>
-__global__ __launch_bounds__(64 * kWavesR) void paged_att_rows(Args a) {
+__global__ __launch_bounds__(64 * kWavesR, 2) void paged_att_rows(Args a) {
   typedef Geo<T, DP> Ge;
-  constexpr int NT = Ge::EB == 2 ? 2 : 1;         // score tiles a step (64 or 32 keys)
-  constexpr int kImg = NT * kKeys * Ge::RB;
-  constexpr int kThreads = 64 * kWavesR;
-  constexpr int kIt = kImg / (16 * kThreads);
-  static_assert(kIt >= 1, "an image holds at least 16 bytes a thread");
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kImg];
+  constexpr int NT = Ge::EB == 2 ? 2 : 1;  // score tiles a step (64 or 32 keys)
+  constexpr int kStep = NT * kKeys;
+  constexpr int kImg = kStep * Ge::RB;
+  constexpr int kIt = kImg / 1024 / kWavesR;  // loads of one image a wave
+  constexpr int kRowsL = kStep / kWavesR;     // image rows a wave loads
+  static_assert(kIt >= 1 && 4 * kImg <= 65536, "load_lds reaches 64 KB");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * kImg];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kh = blockIdx.y;
-  int x = blockIdx.x;
-  const int tile = a.tiles - 1 - x % a.tiles, s = x / a.tiles;  // (the longest tiles of a sequence first)
+  const Job job = job_of(a);
+  const int s = job.s, kh = job.kh, split = job.split;
   if (s >= a.n) {
-    zero_rows(a, tile * a.kvh + kh, a.tiles * a.kvh, Ge::EB);
+    rest_of_rows(a, job, Ge::EB);
     return;
   }
   const Seq q = seq_of(a, s);
-  const int g0 = tile * kTileR;
+  rows_behind(a, job, q);
+  const int g0 = job.tile * kTileR;
   if (g0 >= q.rows * a.G) return;
+  const int ilast = min(q.rows - 1, (g0 + kTileR - 1) / a.G);
+  const int most = a.causal ? max(0, min(q.kv, q.st + ilast + 1)) : q.kv;
+  const Range rg = range_of(a, most, split, kStep);
+  if (split >= rg.used) return;
   const int m0 = g0 + wave * kRowsW;
   const long long seq = a.offsets ? 0 : s;
   const unsigned char* qb = a.q + seq * a.q_seq + q.q0 * a.q_row;
   const unsigned char* kn = a.kn ? a.kn + seq * a.k_seq + q.q0 * a.k_row + (long long)kh * a.k_head : nullptr;
   const unsigned char* vn = a.vn ? a.vn + seq * a.v_seq + q.q0 * a.v_row + (long long)kh * a.v_head : nullptr;
+  const int* tab = a.table + (long long)s * a.width;
+  const int t0 = rg.first / kStep, t1 = (rg.last + kStep - 1) / kStep;
+  const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(lds));
+  if (a.D != DP) {
+    clear_lds<T, DP>(lds, 4 * kImg, tid, 64 * kWavesR);
+    __syncthreads();
+  }
+  const int safe = a.kn ? max(0, min(q.kv, q.st)) : q.kv;
+  Pages pg;
+  uint32_t gaps = 0;  // bit of a buffer: a page of its keys is outside the pool
+  pg.start(a, tab, (t0 * kStep) >> a.sh, lane);
+  const auto issue = [&](int step) {
+    const int j0 = step * kStep;
+    pg.need(a, tab, j0 >> a.sh, (j0 + kStep - 1) >> a.sh, lane);
+    const uint32_t slot = (uint32_t)(step - t0) % 2u, d = at + slot * (2 * kImg);
+    const bool gap = pg.any_bad(j0 >> a.sh, (min(q.kv, j0 + kStep) - 1) >> a.sh);
+    gaps = (gaps & ~(1u << slot)) | ((uint32_t)gap << slot);
+    load_tile<T, DP, kIt>(a, q, pg, kn, vn, kh, j0, wave * kRowsL, safe, d, d + kImg, lane);
+  };
+  if (t0 < t1) issue(t0);
+  if (t0 + 1 < t1) issue(t0 + 1);
   Cols<T, DP> w;
   cols_init<T, DP>(w, a, q, qb, kh, m0, lane);
-  const int ilast = min(q.rows - 1, (g0 + kTileR - 1) / a.G);
-  const int most = a.causal ? max(0, min(q.kv, q.st + ilast + 1)) : q.kv;
-  constexpr int kStep = NT * kKeys;
-  const int nstep = (most + kStep - 1) / kStep;
-  const int* tab = a.table + (long long)s * a.width;
-  const int rb = a.D * Ge::EB, nch = rb / 16;
-  unsigned char *kt = lds, *vt = lds + kImg;
-  uint4 rk[kIt], rv[kIt];
-  uint32_t bad = 0;
   bool odd = false;  // a value that is not finite was scrubbed
   const int least = a.causal ? max(0, min(q.kv, q.st + g0 / a.G + 1)) : q.kv;  // keys the tile's first row sees
-  const auto fetch = [&](int step) {
+  for (int step = t0; step < t1; ++step) {
+    unsigned char* kt = lds + (uint32_t)(step - t0) % 2u * (2 * kImg);
+    unsigned char* vt = kt + kImg;
     const int j0 = step * kStep;
-    bad = 0;
+    if (step + 1 < t1)
+      wait_loads<2 * kIt>();
+    else
+      wait_loads<0>();
+    if (least < min(q.kv, j0 + kStep))
+      odd |= scrub_image<T>(vt + wave * kRowsL * Ge::RB, kRowsL * Ge::RB, lane, 64);  // (what the wave has loaded)
+    wave_barrier();
+    if (!__all(j0 >= w.lim)) {
+      f32x16 sc[NT];
 #pragma unroll
-    for (int t = 0; t < kIt; ++t) {
-      const int ci = t * kThreads + tid;
-      const int row = ci / Ge::NC, cp = ci % Ge::NC, j = j0 + row;
-      const int page = j < q.kv ? tab[j >> a.sh] : -1;
-      RowSrc r;
-      if (!row_src(a, q, kn, vn, kh, j, page, rb, r) && j < q.kv) bad |= 1u;
-      const int ck = cp ^ Ge::k_swz(row & 31), cv = cp ^ Ge::v_swz(row);
-      rk[t] = ck < nch ? *reinterpret_cast<const uint4*>(r.k + ck * 16) : uint4{0, 0, 0, 0};
-      rv[t] = cv < nch ? *reinterpret_cast<const uint4*>(r.v + cv * 16) : uint4{0, 0, 0, 0};
-    }
-  };
-  if (nstep > 0) fetch(0);
-  for (int step = 0; step < nstep; ++step) {
-    // (also: every wave is done with the last tiles)
-    const bool any_bad = __syncthreads_or(bad != 0u);
-    if (least < min(q.kv, (step + 1) * kStep)) {
+      for (int t = 0; t < NT; ++t) sc[t] = scores<T, DP>(w, kt + t * kKeys * Ge::RB, lane);
+      const bool gap = (gaps >> ((uint32_t)(step - t0) % 2u)) & 1u;
+      if (gap || !__all(j0 + kStep <= w.lim)) {
 #pragma unroll
-      for (int t = 0; t < kIt; ++t) odd |= scrub<T>(rv[t]);
-    }
-#pragma unroll
-    for (int t = 0; t < kIt; ++t) {
-      const int ci = t * kThreads + tid;
-      *reinterpret_cast<uint4*>(kt + ci * 16) = rk[t];
-      *reinterpret_cast<uint4*>(vt + ci * 16) = rv[t];
-    }
-    __syncthreads();
-    if (step + 1 < nstep) fetch(step + 1);
-    const int j0 = step * kStep;
-    if (__all(j0 >= w.lim)) continue;  // (nothing of this tile is visible to the wave's rows)
-    f32x16 sc[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) sc[t] = scores<T, DP>(w, kt + t * kKeys * Ge::RB, lane);
-    const bool full = !any_bad && __all(j0 + kStep <= w.lim);
-    if (!full) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        uint32_t there = 0xffffffffu;
-        if (any_bad) {
-          const int j = j0 + t * kKeys + (lane & 31);
-          const int page = j < q.kv ? tab[j >> a.sh] : -1;
-          there = (uint32_t)__ballot((unsigned)page < (unsigned)a.pages);
-        }
-        mask_scores(sc[t], j0 + t * kKeys, w.lim, there, lane);
+        for (int t = 0; t < NT; ++t)
+          mask_scores(sc[t], j0 + t * kKeys, w.lim, gap ? keys_there(a, tab, j0 + t * kKeys, q.kv, lane) : ~0u, lane);
       }
-    }
-    soft_step<T, DP, NT>(w, sc, a.c);
+      soft_step<T, DP, NT>(w, sc, a.c);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) weigh<T, DP>(w, sc[t], vt + t * kKeys * Ge::RB, lane);
+      for (int t = 0; t < NT; ++t) weigh<T, DP>(w, sc[t], vt + t * kKeys * Ge::RB, lane);
+    }
+    wait_lds();
+    wave_barrier();  // (every wave has read the tile: the next loads may overwrite it)
+    if (step + 2 < t1) issue(step + 2);
   }
   if (least < most && __syncthreads_or(odd))
-    add_non_finite<T, DP>(w, a, q, kn, vn, tab, kh, least / kStep * kStep, most, lane);
-  if (a.kn) {
+    add_non_finite<T, DP>(w, a, q, kn, vn, tab, kh, max(t0, least / kStep) * kStep, min(most, t1 * kStep), lane);
+  cols_sum<T, DP>(w);
+  if (a.kn && split == 0) {
     const int i0 = (g0 + a.G - 1) / a.G, i1 = min(q.rows, (g0 + kTileR + a.G - 1) / a.G);
-    write_chunk<T>(a, q, s, kn, vn, kh, i0, i1, tid, kThreads);
+    write_chunk<T>(a, q, s, kn, vn, kh, i0, i1, tid, 64 * kWavesR);
   }
-  cols_store<T, DP>(w, a, q, s, kh, m0, lane);
+  if (rg.used > 1) {
+    cols_part<T, DP>(w, a, q, s, kh, m0, split, rg.used, lane);
+  } else {
+    cols_store<T, DP>(w, a, q, s, kh, m0, lane);
+    if (a.splits > 1) mark_whole(a, q, s, kh, m0, lane);
+  }
 }
 
 struct Plan {
   bool rows_kernel;
-  int tiles, splits, waves;
+  int tiles, splits, waves, range;
 };
 
 Plan plan_of(const mfl_paged_attention_args* p) {
@@ -697,25 +941,33 @@ Plan plan_of(const mfl_paged_attention_args* p) {
   const int64_t G = p->heads / p->kv_heads, M = p->rows * G;
   const int64_t kv = p->max_kv < 1 ? 1 : p->max_kv;
   r.rows_kernel = M > 2 * kRowsW;
-  if (r.rows_kernel) {
-    r.tiles = (int)((M + kTileR - 1) / kTileR);
-    r.splits = 1;
-    r.waves = kWavesR;
-    return r;
+  const int64_t rows = r.rows_kernel ? kTileR : kRowsW, step = r.rows_kernel ? 2 * kKeys : kKeys;
+  r.tiles = (int)((M + rows - 1) / rows);
+  if (r.tiles < 1) r.tiles = 1;
+  r.waves = r.rows_kernel ? kWavesR : kv <= 2 * kKeys ? 1 : 2;
+  // tiles that there are: packed sequences share p->total rows
+  int64_t base = p->n * r.tiles;
+  if (p->offsets) {
+    const int64_t few = (p->total * G + rows - 1) / rows + p->n;
+    if (few < base) base = few;
   }
-  r.tiles = (int)((M + kRowsW - 1) / kRowsW);
-  r.waves = kv <= 2 * kKeys ? 1 : 4;
-  const int64_t base = p->n * p->kv_heads * r.tiles;
-  int64_t sp = base > 0 ? (512 + base - 1) / base : 1;
-  const int64_t most = (kv + 4 * 2 * kKeys - 1) / (4 * 2 * kKeys);
-  if (sp > most) sp = most;
-  if (sp > 256) sp = 256;
+  base *= p->kv_heads;
+  if (base < 1) base = 1;
+  const int64_t least = r.rows_kernel ? 512 : 256;  // keys worth a range of their own
+  int64_t range = kv / ((1024 + base - 1) / base);
+  if (range < least) range = least;
+  range = (range + step - 1) / step * step;
+  int64_t sp = (kv + range - 1) / range;
+  if (sp > 512) sp = 512;
   if (r.waves == 1) sp = 1;
-  r.splits = (int)(sp < 1 ? 1 : sp);
+  r.splits = (int)sp;
+  r.range = (int)range;
   return r;
 }
 
 int dp_of(int64_t dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+
+int64_t slots_of(const mfl_paged_attention_args* p) { return p->offsets ? p->total : p->n * p->rows; }
 
 int eb_of(int64_t dtype) { return dtype == 0 ? 4 : (dtype == 2 || dtype == 3) ? 2 : 0; }
 
@@ -746,27 +998,30 @@ bool check(const mfl_paged_attention_args* p) {
   for (const void* v : al)
     if (reinterpret_cast<uintptr_t>(v) & 15u) return mfl_paged_error("%s: a pointer is not 16-byte aligned", who);
   const int64_t M = p->rows * (p->heads / p->kv_heads);
-  if (p->rows > (1ll << 30) || M > (1ll << 30)) return mfl_paged_error("%s: too many rows", who);
+  if (p->rows > (1ll << 30) || M > (1ll << 30) || p->n > (1ll << 30) || slots_of(p) * p->heads >= (1ll << 31)) return mfl_paged_error("%s: too many rows", who);
   const Plan pl = plan_of(p);
-  if ((p->n + 1) * pl.tiles * pl.splits >= (1ll << 31))
+  if ((p->n + 1) * pl.tiles * pl.splits * p->kv_heads >= (1ll << 31))
     return mfl_paged_error("%s: too many sequences and rows for one launch", who);
   return true;
 }
 
 template <class T, int DP>
 int launch(const Args& a, const Plan& pl, hipStream_t st) {
-  const unsigned seqs = (unsigned)a.n + (a.zero_tail ? 1u : 0u);
-  const dim3 grid(seqs * (unsigned)pl.tiles * (unsigned)pl.splits, (unsigned)a.kvh);
-  if (pl.rows_kernel) {
+  const unsigned seqs = (unsigned)a.n + (a.offsets && (a.zero_tail || pl.splits > 1) ? 1u : 0u);
+  const dim3 grid(seqs * (unsigned)pl.tiles * (unsigned)pl.splits * (unsigned)a.kvh);
+  if (pl.rows_kernel)
     hipLaunchKernelGGL((paged_att_rows<T, DP>), grid, dim3(64 * kWavesR), 0, st, a);
-  } else {
-    if (pl.waves == 1)
-      hipLaunchKernelGGL((paged_att_split<T, DP, 1>), grid, dim3(64), 0, st, a);
+  else if (pl.waves == 1)
+    hipLaunchKernelGGL((paged_att_split<T, DP, 1>), grid, dim3(64), 0, st, a);
+  else
+    hipLaunchKernelGGL((paged_att_split<T, DP, 2>), grid, dim3(128), 0, st, a);
+  if (pl.splits > 1) {
+    const long long rows = a.slots * a.heads;
+    constexpr int kGr = 256 / (DP / 4);
+    if (pl.splits > 16)
+      hipLaunchKernelGGL((paged_att_join<T, DP, true>), dim3((unsigned)rows), dim3(256), 0, st, a);
     else
-      hipLaunchKernelGGL((paged_att_split<T, DP, 4>), grid, dim3(256), 0, st, a);
-    if (pl.splits > 1)
-      hipLaunchKernelGGL((paged_att_join<T, DP>), dim3((unsigned)a.n * (unsigned)pl.tiles, (unsigned)a.kvh), dim3(256),
-                         0, st, a);
+      hipLaunchKernelGGL((paged_att_join<T, DP, false>), dim3((unsigned)((rows + kGr - 1) / kGr)), dim3(256), 0, st, a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
@@ -804,7 +1059,8 @@ int64_t mfl_paged_attention_workspace_bytes(const mfl_paged_attention_args* p) {
   if (!check(p)) return -1;
   const Plan pl = plan_of(p);
   if (pl.splits == 1) return 0;
-  return p->n * p->kv_heads * pl.tiles * pl.splits * (64 + 32 * dp_of(p->dim)) * 4;
+  const int64_t sh = slots_of(p) * p->heads;
+  return ((sh + 3) / 4 * 4 + (pl.splits * sh * 2 + 3) / 4 * 4 + pl.splits * sh * dp_of(p->dim)) * 4;
 }
 
 int mfl_paged_attention(const mfl_paged_attention_args* p, void* stream) {
@@ -818,8 +1074,7 @@ int mfl_paged_attention(const mfl_paged_attention_args* p, void* stream) {
     mfl_paged_error("mfl_paged_attention: NULL pointer");
     return 1;
   }
-  Plan pl = plan_of(p);
-  if (pl.tiles < 1) pl.tiles = 1;
+  const Plan pl = plan_of(p);
   if (pl.splits > 1 && !p->workspace) {
     mfl_paged_error("mfl_paged_attention: NULL workspace");
     return 1;
@@ -852,6 +1107,8 @@ int mfl_paged_attention(const mfl_paged_attention_args* p, void* stream) {
   a.tiles = pl.tiles;
   a.zero_tail = p->offsets && p->zero_tail;
   a.total = p->total;
+  a.slots = slots_of(p);
+  a.range = pl.range;
   a.q_seq = p->q_seq * eb, a.q_row = p->q_row * eb, a.q_head = p->q_head * eb;
   a.k_seq = p->k_seq * eb, a.k_row = p->k_row * eb, a.k_head = p->k_head * eb;
   a.v_seq = p->v_seq * eb, a.v_row = p->v_row * eb, a.v_head = p->v_head * eb;
