@@ -362,11 +362,30 @@ def stream_handle(device):
 _same_device = contextlib.nullcontext()
 
 
-def on_device(device):
-    """Context in which ``device`` is the current one (kernels launch on the current device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _same_device
-    return torch.cuda.device(device)
+def on_device(index):
+    """Context in which device ``index`` is the current one (kernels launch on the current device)."""
+    return _same_device if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def raw_stream(index):
+    """The current stream of device ``index`` as an address."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def device_index(who, named):
+    """The device index of the tensors in ``named`` ((name, tensor or None) pairs): one ROCm device, or an error."""
+    index = None
+    for name, t in named:
+        if t is None:
+            continue
+        i = t.get_device()
+        if i != index:
+            if i < 0:
+                raise RuntimeError(f"{who}: {name} must be a ROCm device tensor (got {t.device}); no CPU implementation")
+            if index is not None:
+                raise ValueError(f"{who}: {name} is on device {i}, the others on {index}")
+            index = i
+    return index
 
 
 _own_streams = {}

@@ -1,12 +1,14 @@
 // Penalties, biases and masks on logits (include/logits_process.h) for gfx950, with the row's best token and
 // log-sum-exp: one pass over the logits, which bound it (each read once, each written once at most).
 //
-// A workgroup takes a tile of one row's vocabulary.  How often each token of the tile occurs in the row's
-// history is counted in LDS (integer atomics: any order gives the same counts) — the history is read once per
-// tile, out of the L2 — and the tile is streamed eight tokens a thread.  The best token is the maximum
-// of 64-bit keys (the value's order-preserving bits above the complement of the index: ties go to the lowest
-// index); the sum of exponentials is kept online in fp32 against a running maximum.  Rows of one tile finish in the same
-// launch, else logits_join merges the tiles' (key, sum) pairs.
+// A workgroup takes a tile of one row's vocabulary, eight tokens a thread, held in registers.  How often each
+// token of the tile occurs in the row's history is counted in LDS (integer atomics: any order gives the same counts);
+// the first of a token's occurrences to be seen again then penalises its logit once and leaves it in LDS, so that
+// the dense pass only picks it up.  The row's history is read once per tile, out of the L2: long histories
+// take tiles of 8,192 tokens (1,024 threads), short ones tiles of 2,048, of which there are more to fill the chip.
+// The best token goes by 64-bit keys (the value's order-preserving bits above the complement of the index: ties go to
+// the lowest index, NaN above all).  Rows of one tile finish in the same launch, else logits_join merges the
+// tiles' (key, sum of exponentials) pairs.
 //
 // The arithmetic is the header's, operation by operation: contraction is off, so that equal logits stay
 // equal and the pick does not depend on what the compiler fuses.
@@ -23,9 +25,10 @@
 
 namespace {
 
-constexpr int kT = 256;
-constexpr int kV = 8;           // tokens a thread takes at a time
-constexpr int kTile = 8192;     // tokens a workgroup (their counts: 32 KB of LDS)
+constexpr int kV = 8;                 // tokens a thread
+constexpr int kFew = 256, kMany = 1024;  // threads a workgroup: short / long histories
+constexpr int kLongHistory = 512;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
   const unsigned char* logits;
@@ -97,32 +100,63 @@ __device__ __forceinline__ float base_of(float m) { return m == -INFINITY || m !
 
 struct Stat {
   unsigned long long key;
-  float m, s;  // running maximum (NaN ignored) and sum of exp(x - base_of(m))
+  float m, s;  // maximum (NaN ignored) and sum of exp(x - base_of(m))
 };
+
+__device__ __forceinline__ float exp_diff(float x, float b) { return __builtin_amdgcn_exp2f((x - b) * kLog2e); }
 
 __device__ __forceinline__ void merge(Stat& a, unsigned long long key, float m, float s) {
   const float mn = fmaxf(a.m, m), b = base_of(mn);
   // (a side that saw nothing has m = -inf and s = 0)
-  a.s = (a.m == -INFINITY ? a.s : a.s * expf(base_of(a.m) - b)) + (m == -INFINITY ? s : s * expf(base_of(m) - b));
+  a.s = (a.m == -INFINITY ? a.s : a.s * exp_diff(base_of(a.m), b)) + (m == -INFINITY ? s : s * exp_diff(base_of(m), b));
   a.m = mn;
   a.key = max_key(a.key, key);
 }
 
-__device__ __forceinline__ Stat block_stat(Stat t) {
-  __shared__ unsigned long long sk[kT / 64];
-  __shared__ float sm[kT / 64], ss[kT / 64];
+// the wave's eight tokens a lane (the first m of them, index v and on)
+__device__ __forceinline__ Stat wave_stat(const float (&x)[kV], int m, int v) {
+  float mx = -INFINITY;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const unsigned long long k = __shfl_xor(t.key, o);
-    const float m = __shfl_xor(t.m, o), s = __shfl_xor(t.s, o);
-    merge(t, k, m, s);
-  }
+  for (int e = 0; e < kV; ++e) mx = fmaxf(mx, e < m ? x[e] : -INFINITY);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+  const float b = base_of(mx);
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < kV; ++e) s += e < m ? exp_diff(x[e], b) : 0.f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  const bool nan = s != s;  // (the base is finite: only a NaN token makes one)
+  int at = -1;
+#pragma unroll
+  for (int e = kV - 1; e >= 0; --e)
+    if (e < m && (nan ? x[e] != x[e] : x[e] == mx)) at = v + e;
+  const unsigned long long who = __ballot(at >= 0);  // (lanes hold ascending tokens)
+  Stat t;
+  t.key = who ? key_of(nan ? NAN : mx, __shfl(at, __builtin_ctzll(who))) : 0ull;
+  t.m = mx;
+  t.s = s;
+  return t;
+}
+
+template <int THREADS>
+__device__ __forceinline__ Stat block_stat(Stat t) {
+  __shared__ unsigned long long sk[THREADS / 64];
+  __shared__ float sm[THREADS / 64], ss[THREADS / 64];
   const int w = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) sk[w] = t.key, sm[w] = t.m, ss[w] = t.s;
   __syncthreads();
-  Stat r{sk[0], sm[0], ss[0]};
+  Stat r{0ull, -INFINITY, 0.f};
+  if (threadIdx.x < 64) {
+    const int i = threadIdx.x;
+    if (i < THREADS / 64) r = Stat{sk[i], sm[i], ss[i]};
 #pragma unroll
-  for (int i = 1; i < kT / 64; ++i) merge(r, sk[i], sm[i], ss[i]);
+    for (int o = THREADS / 128; o > 0; o >>= 1) {
+      const unsigned long long k = __shfl_xor(r.key, o);
+      const float m = __shfl_xor(r.m, o), s = __shfl_xor(r.s, o);
+      merge(r, k, m, s);
+    }
+  }
   return r;
 }
 
@@ -136,107 +170,116 @@ __device__ __forceinline__ void finish(const Args& a, int row, const Stat& r) {
   if (a.logprob) a.logprob[row] = top == -INFINITY ? -INFINITY : top - lse;
 }
 
-template <class T, class O>
-__global__ __launch_bounds__(kT) void logits_tile(Args a) {
-  __shared__ int count[kTile];
+constexpr uint32_t kNone = 0xffffffffu;  // no penalised value (a NaN that the penalties never make)
+
+template <class T, class O, int THREADS>
+__global__ __launch_bounds__(THREADS) void logits_tile(Args a) {
+  constexpr int kTile = THREADS * kV;
+  __shared__ __attribute__((aligned(16))) uint32_t value[kTile];  // penalised logits
+  __shared__ __attribute__((aligned(16))) uint32_t count[kTile];
   const int row = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
   const int v0 = tile * kTile, nv = min(kTile, a.vocab - v0);
+  const int i = threadIdx.x * kV, m = max(0, min(kV, nv - i));
+  const T* src = reinterpret_cast<const T*>(a.logits) + row * a.logits_row + v0;
+  float x[kV], b[kV];
+  uint32_t ok = 0xffu;
+  if (m > 0) {
+    load8(src + i, m, x);
+    if (a.bias) load8(a.bias + row * a.bias_row + v0 + i, m, b);
+    if (a.kind) {
+      const int mr = a.states ? a.states[row] : (a.allowed_rows == 1 ? 0 : row);  // mask row
+      if ((unsigned)mr < (unsigned)a.allowed_rows) {
+        if (a.kind == 2) {
+          // (v0 and i are multiples of 8: the eight bits are one byte of a word)
+          ok = a.allowed[(long long)mr * a.allowed_row * 4 + (v0 + i) / 8];
+        } else {
+          const unsigned char* p = a.allowed + (long long)mr * a.allowed_row + v0 + i;
+          unsigned long long w = 0;
+          if (m == kV) {
+            __builtin_memcpy(&w, p, 8);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kV; ++e)
+              if (e < m) w |= (unsigned long long)p[e] << (8 * e);
+          }
+          ok = 0;
+#pragma unroll
+          for (int e = 0; e < kV; ++e) ok |= ((w >> (8 * e)) & 0xffu ? 1u : 0u) << e;
+        }
+      }
+    }
+  }
   bool any = false;
   if (a.hist > 0) {
-    for (int i = threadIdx.x; i < nv; i += kT) count[i] = 0;
-    __syncthreads();
+    const uint4 none = {kNone, kNone, kNone, kNone}, zero = {0, 0, 0, 0};
+    uint4* vp = reinterpret_cast<uint4*>(value + i);
+    uint4* cp = reinterpret_cast<uint4*>(count + i);
+    vp[0] = none, vp[1] = none;
+    cp[0] = zero, cp[1] = zero;
     const int len = a.token_lens ? max(0, min(a.token_lens[row], a.hist)) : a.hist;
     const int* tok = a.tokens + row * a.tokens_row;
-    for (int i = threadIdx.x; i < len; i += kT) {
-      const int v = tok[i] - v0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < len; j += THREADS) {
+      const int v = tok[j] - v0;
       if ((unsigned)v < (unsigned)nv) {
-        atomicAdd(count + v, 1);
+        atomicAdd(count + v, 1u);
         any = true;
       }
     }
     any = __syncthreads_or(any);
-  }
-  const float rep = a.rep ? a.rep[row] : a.rep_s, pres = a.pres ? a.pres[row] : a.pres_s;
-  const float freq = a.freq ? a.freq[row] : a.freq_s;
-  const T* src = reinterpret_cast<const T*>(a.logits) + row * a.logits_row + v0;
-  O* dst = a.out ? reinterpret_cast<O*>(a.out) + row * a.out_row + v0 : nullptr;
-  const float* bias = a.bias ? a.bias + row * a.bias_row + v0 : nullptr;
-  int mr = -1;  // mask row
-  if (a.kind) {
-    mr = a.states ? a.states[row] : (a.allowed_rows == 1 ? 0 : row);
-    if ((unsigned)mr >= (unsigned)a.allowed_rows) mr = -1;
+    if (any) {
+      const float rep = a.rep ? a.rep[row] : a.rep_s, pres = a.pres ? a.pres[row] : a.pres_s;
+      const float freq = a.freq ? a.freq[row] : a.freq_s;
+      for (int j = threadIdx.x; j < len; j += THREADS) {
+        const int v = tok[j] - v0;
+        if ((unsigned)v >= (unsigned)nv) continue;
+        const uint32_t c = atomicOr(count + v, 0x80000000u);
+        if (c & 0x80000000u) continue;  // (another occurrence has it)
+        const float l = (float)src[v];
+        float y = l > 0.f ? l / rep : l * rep;
+        y = y - pres;
+        y = y - freq * (float)c;
+        value[v] = __float_as_uint(y);
+      }
+      __syncthreads();
+    }
   }
   const bool stats = a.best || a.lse || a.logprob;
-  Stat t{0ull, -INFINITY, 0.f};
-  for (int i = threadIdx.x * kV; i < nv; i += kT * kV) {
-    const int m = min(kV, nv - i);
-    float x[kV];
-    load8(src + i, m, x);
+  if (m > 0) {
     if (any) {
 #pragma unroll
       for (int e = 0; e < kV; ++e) {
-        const int c = e < m ? count[i + e] : 0;
-        if (c > 0) {
-          float y = x[e] > 0.f ? x[e] / rep : x[e] * rep;
-          y = y - pres;
-          x[e] = y - freq * (float)c;
-        }
+        const uint32_t y = value[i + e];
+        x[e] = y == kNone ? x[e] : __uint_as_float(y);
       }
     }
-    if (bias) {
-      float b[kV];
-      load8(bias + i, m, b);
+    if (a.bias) {
 #pragma unroll
       for (int e = 0; e < kV; ++e) x[e] = x[e] + b[e];
     }
-    if (mr >= 0) {
-      uint32_t ok = 0;
-      if (a.kind == 2) {
-        // (v0 and i are multiples of 8: the eight bits are one byte of the word, in range with it)
-        ok = a.allowed[(long long)mr * a.allowed_row * 4 + (v0 + i) / 8];
-      } else {
-        const unsigned char* p = a.allowed + (long long)mr * a.allowed_row + v0 + i;
 #pragma unroll
-        for (int e = 0; e < kV; ++e) ok |= (e < m && p[e] != 0 ? 1u : 0u) << e;
-      }
+    for (int e = 0; e < kV; ++e) x[e] = (ok >> e) & 1u ? x[e] : -INFINITY;
+    if (a.out) store8(reinterpret_cast<O*>(a.out) + row * a.out_row + v0 + i, m, x);
+  } else {
 #pragma unroll
-      for (int e = 0; e < kV; ++e) x[e] = (ok >> e) & 1u ? x[e] : -INFINITY;
-    }
-    if (dst) store8(dst + i, m, x);
-    if (stats) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < kV; ++e)
-        if (e < m) {
-          mx = fmaxf(mx, x[e]);
-          t.key = max_key(t.key, key_of(x[e], v0 + i + e));
-        }
-      if (mx > t.m) {
-        if (t.m != -INFINITY) t.s *= expf(base_of(t.m) - base_of(mx));
-        t.m = mx;
-      }
-      const float b = base_of(t.m);
-#pragma unroll
-      for (int e = 0; e < kV; ++e)
-        if (e < m) t.s += expf(x[e] - b);
-    }
+    for (int e = 0; e < kV; ++e) x[e] = -INFINITY;
   }
   if (!stats) return;
-  const Stat r = block_stat(t);
+  const Stat r = block_stat<THREADS>(wave_stat(x, m, v0 + i));
   if (threadIdx.x != 0) return;
   if (a.tiles == 1) {
     finish(a, row, r);
   } else {
     a.keys[(long long)row * a.tiles + tile] = r.key;
-    // the sum against the tile's own maximum, which the key holds (NaN: the sum is NaN already)
+    // the sum against the tile's own maximum, which the key holds (with a NaN the sum is NaN)
     a.sums[(long long)row * a.tiles + tile] = r.s;
   }
 }
 
-__global__ __launch_bounds__(kT) void logits_join(Args a) {
+__global__ __launch_bounds__(64) void logits_join(Args a) {
   const int row = blockIdx.x;
   Stat t{0ull, -INFINITY, 0.f};
-  for (int i = threadIdx.x; i < a.tiles; i += kT) {
+  for (int i = threadIdx.x; i < a.tiles; i += 64) {
     const unsigned long long k = a.keys[(long long)row * a.tiles + i];
     const float m = key_value(k), s = a.sums[(long long)row * a.tiles + i];
     if (m != m) {  // a NaN: the row's sum is one whatever the others hold
@@ -246,8 +289,13 @@ __global__ __launch_bounds__(kT) void logits_join(Args a) {
       merge(t, k, m, s);
     }
   }
-  const Stat r = block_stat(t);
-  if (threadIdx.x == 0) finish(a, row, r);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const unsigned long long k = __shfl_xor(t.key, o);
+    const float m = __shfl_xor(t.m, o), s = __shfl_xor(t.s, o);
+    merge(t, k, m, s);
+  }
+  if (threadIdx.x == 0) finish(a, row, t);
 }
 
 thread_local char g_err[256] = "";
@@ -262,7 +310,12 @@ bool bad(const char* fmt, ...) {
 
 int esize(int64_t t) { return t == 0 ? 4 : t == 2 || t == 3 ? 2 : 0; }
 
-int tiles_of(const mfl_logits_args* p) { return (int)((p->vocab + kTile - 1) / kTile); }
+int threads_of(const mfl_logits_args* p) { return p->hist > kLongHistory ? kMany : kFew; }
+
+int tiles_of(const mfl_logits_args* p) {
+  const int64_t tile = (int64_t)threads_of(p) * kV;
+  return (int)((p->vocab + tile - 1) / tile);
+}
 
 bool check(const mfl_logits_args* p) {
   const char* who = "mfl_logits_process";
@@ -286,15 +339,23 @@ bool check(const mfl_logits_args* p) {
   return true;
 }
 
-template <class T>
-void launch(const Args& a, int64_t out_dtype, hipStream_t st) {
+template <class T, class O>
+void launch_out(const Args& a, int threads, hipStream_t st) {
   const dim3 grid((unsigned)a.n * (unsigned)a.tiles);
-  if (out_dtype == 0)
-    hipLaunchKernelGGL((logits_tile<T, float>), grid, dim3(kT), 0, st, a);
-  else if (out_dtype == 2)
-    hipLaunchKernelGGL((logits_tile<T, __bf16>), grid, dim3(kT), 0, st, a);
+  if (threads == kMany)
+    hipLaunchKernelGGL((logits_tile<T, O, kMany>), grid, dim3(kMany), 0, st, a);
   else
-    hipLaunchKernelGGL((logits_tile<T, _Float16>), grid, dim3(kT), 0, st, a);
+    hipLaunchKernelGGL((logits_tile<T, O, kFew>), grid, dim3(kFew), 0, st, a);
+}
+
+template <class T>
+void launch(const Args& a, int64_t out_dtype, int threads, hipStream_t st) {
+  if (out_dtype == 0)
+    launch_out<T, float>(a, threads, st);
+  else if (out_dtype == 2)
+    launch_out<T, __bf16>(a, threads, st);
+  else
+    launch_out<T, _Float16>(a, threads, st);
 }
 
 }  // namespace
@@ -346,12 +407,12 @@ int mfl_logits_process(const mfl_logits_args* p, void* stream) {
   a.rep_s = (float)p->repetition, a.pres_s = (float)p->presence, a.freq_s = (float)p->frequency;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (p->dtype == 0)
-    launch<float>(a, p->out_dtype, st);
+    launch<float>(a, p->out_dtype, threads_of(p), st);
   else if (p->dtype == 2)
-    launch<__bf16>(a, p->out_dtype, st);
+    launch<__bf16>(a, p->out_dtype, threads_of(p), st);
   else
-    launch<_Float16>(a, p->out_dtype, st);
-  if (tiles > 1 && stats) hipLaunchKernelGGL(logits_join, dim3((unsigned)a.n), dim3(kT), 0, st, a);
+    launch<_Float16>(a, p->out_dtype, threads_of(p), st);
+  if (tiles > 1 && stats) hipLaunchKernelGGL(logits_join, dim3((unsigned)a.n), dim3(64), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
     bad("mfl_logits_process: launch failed: %s", hipGetErrorString(e));

@@ -92,26 +92,17 @@ def _run(who, logits, tokens, token_lens, repetition, presence, frequency, bias,
     if out is not None and (tuple(out.shape) != (n, vocab) or out.dtype not in _DTYPES or
                             (vocab > 1 and out.stride(1) != 1)):
         raise ValueError(f"{who}: out must be ({n}, {vocab}) with contiguous rows, float32, bfloat16 or float16")
-    dev = None
-    for name, t in (("logits", logits), ("tokens", tokens), ("token_lens", token_lens), ("repetition", rep_t),
-                    ("presence", pres_t), ("frequency", freq_t), ("bias", bias), ("allowed", allowed),
-                    ("states", states), ("out", out)):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"{who}: {name} must be a ROCm device tensor (got {t.device}); no CPU implementation")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{who}: {name} is on {t.device}, the others on {dev}")
+    dev = _native.device_index(who, (("logits", logits), ("tokens", tokens), ("token_lens", token_lens),
+                                     ("repetition", rep_t), ("presence", pres_t), ("frequency", freq_t), ("bias", bias),
+                                     ("allowed", allowed), ("states", states), ("out", out)))
     if out is not logits and vocab > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
     lib = _native.load_library()
     with _native.on_device(dev):
         if write and out is None:
-            out = torch.empty(n, vocab, dtype=torch.float32, device=dev)
-        best = torch.empty(n, dtype=torch.int64, device=dev) if stats else None
-        rest = torch.empty(n, dtype=torch.float32, device=dev) if stats else None
+            out = torch.empty(n, vocab, dtype=torch.float32, device=logits.device)
+        best = torch.empty(n, dtype=torch.int64, device=logits.device) if stats else None
+        rest = torch.empty(n, dtype=torch.float32, device=logits.device) if stats else None
 
         def ptr(t):
             return 0 if t is None else t.data_ptr()
@@ -125,9 +116,9 @@ def _run(who, logits, tokens, token_lens, repetition, presence, frequency, bias,
         args = _ARGS.pack(*head, 0, *tail)
         need = lib.mfl_logits_workspace_bytes(args)
         if need > 0:
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
             args = _ARGS.pack(*head, ws.data_ptr(), *tail)
-        if need < 0 or lib.mfl_logits_process(args, _native.stream_handle(dev)) != 0:
+        if need < 0 or lib.mfl_logits_process(args, _native.raw_stream(dev)) != 0:
             raise RuntimeError(f"{who}: " + lib.mfl_logits_last_error().decode(errors="replace"))
     return out, best, rest
 

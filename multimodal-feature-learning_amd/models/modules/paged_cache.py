@@ -26,20 +26,6 @@ def _error(who):
     raise RuntimeError(f"{who}: " + _native.load_library().mfl_paged_last_error().decode(errors="replace"))
 
 
-def _device(who, **tensors):
-    dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"{who}: {name} must be a ROCm device tensor (got {t.device}); no CPU implementation")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{who}: {name} is on {t.device}, the others on {dev}")
-    return dev
-
-
 def _i32(who, name, t, shape):
     if t.dtype != torch.int32:
         raise TypeError(f"{who}: {name} must be int32, got {t.dtype}")
@@ -49,12 +35,17 @@ def _i32(who, name, t, shape):
 
 
 def _rows16(t):
-    """t with a contiguous last dimension, 16-byte aligned rows and start (copied only when it has not)."""
-    e = 16 // t.element_size()
+    """(t, its strides) with a contiguous last dimension, 16-byte aligned rows and start (copied only if it has not)."""
     st = t.stride()
-    if st[-1] != 1 or t.data_ptr() % 16 or any(s % e for s, n in zip(st[:-1], t.shape) if n > 1):
-        return t.contiguous() if not t.is_contiguous() else t.clone()
-    return t
+    mask = 16 // t.element_size() - 1
+    if t.data_ptr() % 16 == 0 and st[-1] == 1:
+        if not (st[-2] | st[-3] | st[0]) & mask:
+            return t, st
+        st = tuple(0 if n == 1 else x for x, n in zip(st, t.shape))  # (a dimension of one may have any stride)
+        if not (st[-2] | st[-3] | st[0]) & mask:
+            return t, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
 
 
 def paged_attention(q, k_pages, v_pages, table, kv_lens, *, k=None, v=None, starts=None, offsets=None, max_rows=None,
@@ -91,9 +82,10 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, *, k=None, v=None, star
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
         raise ValueError(f"{who}: k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must be (pages, "
                          "kv_heads, page_size, dim)")
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("k", k), ("v", v)):
-        if t is not None and t.dtype != q.dtype:
-            raise TypeError(f"{who}: {name} is {t.dtype}, q {q.dtype}")
+    dt = q.dtype
+    if k_pages.dtype != dt or v_pages.dtype != dt or k is not None and (k.dtype != dt or v.dtype != dt):
+        raise TypeError(f"{who}: pages, k and v must be {dt} like q; got {k_pages.dtype}, {v_pages.dtype}"
+                        + ("" if k is None else f", {k.dtype}, {v.dtype}"))
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError(f"{who}: pages must be contiguous")
     pages, kvh, ps, d = k_pages.shape
@@ -106,7 +98,8 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, *, k=None, v=None, star
     if table.dim() != 2:
         raise ValueError(f"{who}: table must be (n, width); got {tuple(table.shape)}")
     n, width = table.shape
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k_pages, v_pages, k, v)):
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad
+                                    or k is not None and (k.requires_grad or v.requires_grad)):
         raise RuntimeError(f"{who}: inference only (no gradient); call it under torch.no_grad()")
     table = _i32(who, "table", table, (n, width))
     kv_lens = _i32(who, "kv_lens", kv_lens, (n,))
@@ -124,19 +117,19 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, *, k=None, v=None, star
         raise ValueError(f"{who}: max_rows {max_rows}")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError(f"{who}: out must be a contiguous {tuple(q.shape)} {q.dtype} tensor")
-    dev = _device(who, q=q, k_pages=k_pages, v_pages=v_pages, k=k, v=v, table=table, kv_lens=kv_lens, starts=starts,
-                  offsets=offsets, out=out)
+    dev = _native.device_index(who, (("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("k", k), ("v", v),
+                                     ("table", table), ("kv_lens", kv_lens), ("starts", starts), ("offsets", offsets),
+                                     ("out", out)))
     zero_tail = packed and out is None
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    q = _rows16(q)
-    qs = q.stride()
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    q, qs = _rows16(q)
     if k is None:
         kp = vp = 0
         ks = vs = (0, 0, 0, 0)
     else:
-        k, v = _rows16(k), _rows16(v)
-        kp, vp, ks, vs = k.data_ptr(), v.data_ptr(), k.stride(), v.stride()
+        (k, ks), (v, vs) = _rows16(k), _rows16(v)
+        kp, vp = k.data_ptr(), v.data_ptr()
     if packed:
         qs, ks, vs = (0,) + qs, (0,) + ks[-3:], (0,) + vs[-3:]
     capacity = width * ps
@@ -152,9 +145,9 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, *, k=None, v=None, star
         _error(who)
     with _native.on_device(dev):
         if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
             args = _ARGS.pack(*ptrs, ws.data_ptr(), *fixed)
-        if lib.mfl_paged_attention(args, _native.stream_handle(dev)) != 0:
+        if lib.mfl_paged_attention(args, _native.raw_stream(dev)) != 0:
             _error(who)
     return out
 
@@ -209,18 +202,19 @@ def pages_update(data, table, lens, refs, *, parents=None, new_lens=None, page_s
         parents = _i32(who, "parents", parents, (n,))
     if new_lens is not None:
         new_lens = _i32(who, "new_lens", new_lens, (n,))
-    dev = _device(who, table=table, lens=lens, refs=refs, parents=parents, new_lens=new_lens, data=data)
+    dev = _native.device_index(who, (("table", table), ("lens", lens), ("refs", refs), ("parents", parents),
+                                     ("new_lens", new_lens), ("data", data)))
     lib = _native.load_library()
     need = lib.mfl_pages_update_workspace_bytes(n, pages)
     with _native.on_device(dev):
         table_out, lens_out, refs_out = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
-        short = torch.empty(1, dtype=torch.int32, device=dev)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        short = torch.empty(1, dtype=torch.int32, device=table.device)
+        ws = torch.empty(need, dtype=torch.uint8, device=table.device)
         if lib.mfl_pages_update(table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
                                 None if parents is None else parents.data_ptr(),
                                 None if new_lens is None else new_lens.data_ptr(), n, width, pages, page_size, ptr or None,
                                 planes, heads, row, table_out.data_ptr(), lens_out.data_ptr(), refs_out.data_ptr(),
-                                short.data_ptr(), ws.data_ptr(), _native.stream_handle(dev)) != 0:
+                                short.data_ptr(), ws.data_ptr(), _native.raw_stream(dev)) != 0:
             _error(who)
     return table_out, lens_out, refs_out, short
 
@@ -245,15 +239,15 @@ def pages_compact(data, table, refs):
         page_bytes = heads * data.shape[4] * row
     table = _i32(who, "table", table, tuple(table.shape))
     refs = _i32(who, "refs", refs, (pages,))
-    dev = _device(who, table=table, refs=refs, data=data)
+    dev = _native.device_index(who, (("table", table), ("refs", refs), ("data", data)))
     lib = _native.load_library()
     with _native.on_device(dev):
         table_out, refs_out, remap = torch.empty_like(table), torch.empty_like(refs), torch.empty_like(refs)
-        live = torch.empty(1, dtype=torch.int32, device=dev)
-        ws = torch.empty(lib.mfl_pages_compact_workspace_bytes(pages), dtype=torch.uint8, device=dev)
+        live = torch.empty(1, dtype=torch.int32, device=table.device)
+        ws = torch.empty(lib.mfl_pages_compact_workspace_bytes(pages), dtype=torch.uint8, device=table.device)
         if lib.mfl_pages_compact(table.data_ptr(), table.numel(), refs.data_ptr(), pages, ptr or None, planes,
                                  page_bytes, table_out.data_ptr(), refs_out.data_ptr(), remap.data_ptr(),
-                                 live.data_ptr(), ws.data_ptr(), _native.stream_handle(dev)) != 0:
+                                 live.data_ptr(), ws.data_ptr(), _native.raw_stream(dev)) != 0:
             _error(who)
     return table_out, refs_out, remap, live
 
@@ -270,11 +264,11 @@ def pages_copy(data, src, dst):
         raise ValueError(f"{who}: src must be (count,); got {tuple(src.shape)}")
     src = _i32(who, "src", src, (src.shape[0],))
     dst = _i32(who, "dst", dst, (src.shape[0],))
-    dev = _device(who, data=data, src=src, dst=dst)
+    dev = _native.device_index(who, (("data", data), ("src", src), ("dst", dst)))
     lib = _native.load_library()
     with _native.on_device(dev):
         if lib.mfl_pages_copy(src.data_ptr(), dst.data_ptr(), src.shape[0], ptr, planes, data.shape[2],
-                              heads * data.shape[4] * row, _native.stream_handle(dev)) != 0:
+                              heads * data.shape[4] * row, _native.raw_stream(dev)) != 0:
             _error(who)
     return data
 
