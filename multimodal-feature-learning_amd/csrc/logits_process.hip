@@ -28,6 +28,7 @@ namespace {
 constexpr int kV = 8;                 // tokens a thread
 constexpr int kFew = 256, kMany = 1024;  // threads a workgroup: short / long histories
 constexpr int kLongHistory = 512;
+constexpr int kTok = 4;               // tokens of the history a thread holds
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -181,6 +182,15 @@ __global__ __launch_bounds__(THREADS) void logits_tile(Args a) {
   const int v0 = tile * kTile, nv = min(kTile, a.vocab - v0);
   const int i = threadIdx.x * kV, m = max(0, min(kV, nv - i));
   const T* src = reinterpret_cast<const T*>(a.logits) + row * a.logits_row + v0;
+  // the history's first kTok tokens a thread stay in registers, fetched with the logits
+  const int len = a.hist == 0 ? 0 : a.token_lens ? max(0, min(a.token_lens[row], a.hist)) : a.hist;
+  const int* tok = a.tokens + row * a.tokens_row;
+  int held[kTok];
+#pragma unroll
+  for (int t = 0; t < kTok; ++t) {
+    const int j = t * THREADS + (int)threadIdx.x;
+    held[t] = j < len ? tok[j] : -1;
+  }
   float x[kV], b[kV];
   uint32_t ok = 0xffu;
   if (m > 0) {
@@ -210,37 +220,39 @@ __global__ __launch_bounds__(THREADS) void logits_tile(Args a) {
     }
   }
   bool any = false;
-  if (a.hist > 0) {
+  if (len > 0) {
     const uint4 none = {kNone, kNone, kNone, kNone}, zero = {0, 0, 0, 0};
     uint4* vp = reinterpret_cast<uint4*>(value + i);
     uint4* cp = reinterpret_cast<uint4*>(count + i);
     vp[0] = none, vp[1] = none;
     cp[0] = zero, cp[1] = zero;
-    const int len = a.token_lens ? max(0, min(a.token_lens[row], a.hist)) : a.hist;
-    const int* tok = a.tokens + row * a.tokens_row;
     __syncthreads();
-    for (int j = threadIdx.x; j < len; j += THREADS) {
-      const int v = tok[j] - v0;
+    const auto add = [&](int v) {
       if ((unsigned)v < (unsigned)nv) {
         atomicAdd(count + v, 1u);
         any = true;
       }
-    }
+    };
+#pragma unroll
+    for (int t = 0; t < kTok; ++t) add(held[t] - v0);
+    for (int j = kTok * THREADS + threadIdx.x; j < len; j += THREADS) add(tok[j] - v0);
     any = __syncthreads_or(any);
     if (any) {
       const float rep = a.rep ? a.rep[row] : a.rep_s, pres = a.pres ? a.pres[row] : a.pres_s;
       const float freq = a.freq ? a.freq[row] : a.freq_s;
-      for (int j = threadIdx.x; j < len; j += THREADS) {
-        const int v = tok[j] - v0;
-        if ((unsigned)v >= (unsigned)nv) continue;
+      const auto apply = [&](int v) {
+        if ((unsigned)v >= (unsigned)nv) return;
         const uint32_t c = atomicOr(count + v, 0x80000000u);
-        if (c & 0x80000000u) continue;  // (another occurrence has it)
+        if (c & 0x80000000u) return;  // (another occurrence has it)
         const float l = (float)src[v];
         float y = l > 0.f ? l / rep : l * rep;
         y = y - pres;
         y = y - freq * (float)c;
         value[v] = __float_as_uint(y);
-      }
+      };
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) apply(held[t] - v0);
+      for (int j = kTok * THREADS + threadIdx.x; j < len; j += THREADS) apply(tok[j] - v0);
       __syncthreads();
     }
   }

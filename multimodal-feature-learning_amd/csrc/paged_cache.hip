@@ -2,12 +2,15 @@
 // copy on write, freeing and compaction decided on the device, so that a decode loop never waits for the host.
 //
 // Everything that decides is integer work whose result does not depend on the order it runs in: reference
-// counts by integer atomics, ranks by prefix sums over fixed blocks.  The order of the rules in the header is a
-// chain of dependences over the whole pool, so each link is a launch:
-//   update_start   refs' = refs, marks cleared             update_refs    rows' pages subtracted / added
-//   update_marks   growing rows marked on shared pages;    update_rank    free pages listed in ascending order;
-//                  free pages counted a block                             the rows' requests numbered
-//   update_commit  the new table and counts; the copies of the used tokens in every plane
+// counts by integer atomics, ranks by prefix sums over fixed blocks.  The header's rules are a chain of dependences
+// over the whole pool: small pools (up to 8,192 pages) are decided by every workgroup for itself in its LDS, in one
+// launch with the copies (update_small); for larger ones each link is a launch:
+//   update_start   counts' = refs, marks cleared
+//   update_refs    the pages that a row had and does not keep, or keeps and had not, subtracted / added
+//                  (beams mostly continue rows that share their pages: nothing to do); growing rows marked
+//   update_count   free pages counted a block; the rows' requests numbered
+//   update_commit  the new table (a row finds its own free pages: block by the counts, then by rank), the new
+//                  reference counts, and the copies of the used tokens in every plane
 // and for the compaction: compact_count, compact_rank, compact_commit.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -20,16 +23,18 @@ namespace {
 constexpr int kT = 256;          // threads a workgroup
 constexpr int kBlock = 1024;     // pages whose free (live) count is one block sum
 constexpr int kCopyWgs = 2048;   // workgroups that share the copies (8 a CU)
+constexpr int kSmallT = 1024;    // update_small: threads, and rows at most
+constexpr int kSmallPages = 8192, kSmallEntries = 16384, kSmallWgs = 256;
 
 struct Row {
-  int keep, total, kept, page;  // tokens kept, new length, pages kept, shared partial last page (-1: none)
+  int keep, total, kept, page;  // tokens kept, new length, pages kept, partial last page of a growing row (or -1)
 };
 
 struct Upd {
   const int *table, *lens, *refs, *parents, *new_lens;
   int n, width, pages, ps, sh, blocks;
   int *table_out, *lens_out, *refs_out, *short_out;
-  int *growing, *highest, *counts, *pool, *first, *cow;  // workspace (first: n + 1, the last the total)
+  int *held, *growing, *highest, *counts, *first, *cow;  // workspace (first: n + 1, the last the total)
   unsigned char* data;
   int planes, heads, rb;
 };
@@ -58,10 +63,184 @@ __device__ __forceinline__ Row row_of(const Upd& a, int s, int p) {
   return r;
 }
 
+// how many of page x's growing rows take a copy (its references: held)
+__device__ __forceinline__ int copies_of(int held, int growing) {
+  return held > 1 ? (growing == held ? growing - 1 : growing) : 0;
+}
+__device__ __forceinline__ bool takes_copy(int held, int growing, int highest, int s) {
+  return held > 1 && !(growing == held && highest == s);
+}
+
+__device__ __forceinline__ void copy16(unsigned char* dst, const unsigned char* src) {
+  *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+}
+
+// the used tokens of page src to page dst in planes pl0 .. pl0 + planes - 1
+__device__ __forceinline__ void copy_used(const Upd& a, int pl0, int planes, int src, int dst, int keep, int tid,
+                                          int threads) {
+  const long long head_bytes = (long long)a.ps * a.rb, page = head_bytes * a.heads;
+  const int used = (keep & (a.ps - 1)) * a.rb / 16;  // 16-byte chunks a head
+  for (long long i = tid; i < (long long)planes * a.heads * used; i += threads) {
+    const long long hd = i / used;
+    const int pl = pl0 + (int)(hd / a.heads);
+    unsigned char* base = a.data + pl * (page * a.pages);
+    const long long off = hd % a.heads * head_bytes + i % used * 16;
+    copy16(base + dst * page + off, base + src * page + off);
+  }
+}
+
+// sum over the workgroup
+template <int THREADS>
+__device__ __forceinline__ int block_sum(int v) {
+  __shared__ int part[THREADS / 64];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  int t = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) t += part[i];
+  return t;
+}
+
+// exclusive prefix over the workgroup's threads; total: the sum
+template <int THREADS, class I>
+__device__ __forceinline__ I block_scan(I v, I& total) {
+  __shared__ I part[THREADS / 64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  I inc = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const I u = __shfl_up(inc, o);
+    if (lane >= o) inc += u;
+  }
+  __syncthreads();
+  if (lane == 63) part[w] = inc;
+  __syncthreads();
+  I before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) {
+    if (i < w) before += part[i];
+    total += part[i];
+  }
+  return before + inc - v;
+}
+
+// sums that may pass 2^31 (requests of all rows) are kept there: only "more than the pool" matters
+__device__ __forceinline__ int clamp_sum(long long v) { return (int)min(v, (long long)INT32_MAX); }
+
+// the state as it was
+__device__ __forceinline__ void keep_state(const Upd& a, int wg, int wgs, int threads) {
+  const long long tid = (long long)wg * threads + threadIdx.x, all = (long long)wgs * threads;
+  for (long long e = tid; e < (long long)a.n * a.width; e += all) a.table_out[e] = a.table[e];
+  for (long long e = tid; e < a.pages; e += all) a.refs_out[e] = a.refs[e];
+  for (long long e = tid; e < a.n; e += all) a.lens_out[e] = a.lens[e];
+}
+
+// n <= kSmallT, pages <= kSmallPages, n * width <= kSmallEntries.  Every workgroup decides all, writes its share of
+// the outputs and does its share of the copies
+__global__ __launch_bounds__(kSmallT) void update_small(Upd a) {
+  extern __shared__ int lds[];
+  int *held = lds, *growing = held + a.pages, *highest = growing + a.pages;  // highest: later the pages asked for
+  __shared__ int s_keep[kSmallT], s_total[kSmallT], s_parent[kSmallT], s_first[kSmallT], s_cow[kSmallT];
+  const int tid = threadIdx.x, wg = blockIdx.x, wgs = gridDim.x;
+  for (int x = tid; x < a.pages; x += kSmallT) {
+    held[x] = a.refs[x];
+    growing[x] = 0;
+    highest[x] = -1;
+  }
+  Row r{0, 0, 0, -1};
+  int p = -1, old_len = 0;
+  if (tid < a.n) {
+    p = parent_of(a, tid);
+    r = row_of(a, tid, p);
+    old_len = clamp_len(a, a.lens[tid]);
+    s_keep[tid] = r.keep;
+    s_total[tid] = r.total;
+    s_parent[tid] = p;
+    s_first[tid] = old_len;  // (until the requests are numbered)
+  }
+  __syncthreads();
+  for (int e = tid; e < a.n * a.width; e += kSmallT) {
+    const int s = e / a.width, c = e - s * a.width;
+    const int q = s_parent[s];
+    const int had = c < pages_of(s_first[s], a.sh) ? a.table[e] : -1;
+    const int has = c < pages_of(s_keep[s], a.sh) ? a.table[q * a.width + c] : -1;
+    if (had == has) continue;
+    if ((unsigned)had < (unsigned)a.pages) atomicSub(held + had, 1);
+    if ((unsigned)has < (unsigned)a.pages) atomicAdd(held + has, 1);
+  }
+  if (r.page >= 0) {
+    atomicAdd(growing + r.page, 1);
+    atomicMax(highest + r.page, tid);
+  }
+  __syncthreads();
+  int cow = 0, need = 0;
+  if (tid < a.n) {
+    cow = r.page >= 0 && takes_copy(held[r.page], growing[r.page], highest[r.page], tid);
+    need = pages_of(r.total, a.sh) - r.kept + cow;
+  }
+  // (need <= kSmallEntries + 1 over kSmallT rows: the sum fits)
+  int asked;
+  const int first = block_scan<kSmallT>(need, asked);
+  // the free pages: each thread ranks a run of them
+  const int run = (a.pages + kSmallT - 1) / kSmallT, x0 = min(a.pages, tid * run), x1 = min(a.pages, x0 + run);
+  int mine = 0;
+  for (int x = x0; x < x1; ++x) mine += held[x] == 0;
+  int free;
+  int rank = block_scan<kSmallT>(mine, free);  // (its barriers: every row has read `highest`)
+  const bool ok = asked <= free;
+  if (wg == 0 && tid == 0) a.short_out[0] = ok ? 0 : asked - free;
+  if (!ok) {
+    keep_state(a, wg, wgs, kSmallT);
+    return;
+  }
+  int* pool = highest;
+  for (int x = x0; x < x1; ++x) {
+    if (held[x] != 0) continue;
+    if (rank < asked) {
+      pool[rank] = x;
+      growing[x] = -1;  // (asked for; no row grows in a free page)
+    }
+    ++rank;
+  }
+  if (tid < a.n) {
+    s_first[tid] = first;
+    s_cow[tid] = cow ? r.page : -1;
+    if (wg == 0) a.lens_out[tid] = r.total;
+  }
+  __syncthreads();
+  for (int x = wg * kSmallT + tid; x < a.pages; x += wgs * kSmallT)
+    a.refs_out[x] = growing[x] < 0 ? 1 : held[x] - copies_of(held[x], growing[x]);
+  for (int e = wg * kSmallT + tid; e < a.n * a.width; e += wgs * kSmallT) {
+    const int s = e / a.width, c = e - s * a.width;
+    const int kept = pages_of(s_keep[s], a.sh), own = s_cow[s] >= 0;
+    int x = -1;
+    if (own && c == kept - 1) {
+      x = pool[s_first[s]];
+    } else if (c < kept) {
+      x = a.table[s_parent[s] * a.width + c];
+      if ((unsigned)x >= (unsigned)a.pages) x = -1;
+    } else if (c < pages_of(s_total[s], a.sh)) {
+      x = pool[s_first[s] + own + c - kept];
+    }
+    a.table_out[e] = x;
+  }
+  if (!a.data) return;
+  // a quarter of the workgroup takes a row's copy in one plane
+  const int part = tid >> 8, lane = tid & 255;
+  for (int e = wg * 4 + part; e < a.n * a.planes; e += wgs * 4) {
+    const int s = e / a.planes, pl = e - s * a.planes;
+    if (s_cow[s] >= 0) copy_used(a, pl, 1, s_cow[s], pool[s_first[s]], s_keep[s], lane, 256);
+  }
+}
+
 __global__ __launch_bounds__(kT) void update_start(Upd a) {
   const int x = blockIdx.x * kT + threadIdx.x;
   if (x >= a.pages) return;
-  a.refs_out[x] = a.refs[x];
+  a.held[x] = a.refs[x];
   a.growing[x] = 0;
   a.highest[x] = -1;
 }
@@ -72,174 +251,123 @@ __global__ __launch_bounds__(kT) void update_refs(Upd a) {
   for (int s = blockIdx.y; s < a.n; s += gridDim.y) {
     const int p = parent_of(a, s);
     const Row r = row_of(a, s, p);
-    const int held = pages_of(clamp_len(a, a.lens[s]), a.sh);
-    const int same = p == s ? min(held, r.kept) : 0;  // pages the row had and keeps
-    if (c < held && c >= same) {
-      const int x = a.table[(long long)s * a.width + c];
-      if ((unsigned)x < (unsigned)a.pages) atomicSub(a.refs_out + x, 1);
+    const int len = pages_of(clamp_len(a, a.lens[s]), a.sh);
+    if (c == 0 && r.page >= 0) {
+      atomicAdd(a.growing + r.page, 1);
+      atomicMax(a.highest + r.page, s);
     }
-    if (c < r.kept && c >= same) {
-      const int x = a.table[(long long)p * a.width + c];
-      if ((unsigned)x < (unsigned)a.pages) atomicAdd(a.refs_out + x, 1);
-    }
+    const int had = c < len ? a.table[(long long)s * a.width + c] : -1;
+    const int has = c < r.kept ? a.table[(long long)p * a.width + c] : -1;
+    if (had == has) continue;
+    if ((unsigned)had < (unsigned)a.pages) atomicSub(a.held + had, 1);
+    if ((unsigned)has < (unsigned)a.pages) atomicAdd(a.held + has, 1);
   }
 }
 
-__device__ __forceinline__ int block_sum(int v) {
-  __shared__ int part[kT / 64];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  int t = 0;
-#pragma unroll
-  for (int i = 0; i < kT / 64; ++i) t += part[i];
-  __syncthreads();
-  return t;
-}
-
-// exclusive prefix over the workgroup's threads; total: the sum
-__device__ __forceinline__ int block_scan(int v, int& total) {
-  __shared__ int part[kT / 64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int inc = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(inc, o);
-    if (lane >= o) inc += u;
-  }
-  if (lane == 63) part[w] = inc;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < kT / 64; ++i) {
-    if (i < w) before += part[i];
-    total += part[i];
-  }
-  __syncthreads();
-  return before + inc - v;
-}
-
-// workgroups 0 .. blocks-1 count the free pages of their block, the others mark rows
-__global__ __launch_bounds__(kT) void update_marks(Upd a) {
+// workgroups 0 .. blocks-1 count the free pages of their block, the last one numbers the rows' requests
+__global__ __launch_bounds__(kT) void update_count(Upd a) {
   if ((int)blockIdx.x < a.blocks) {
     int v = 0;
     for (int i = threadIdx.x; i < kBlock; i += kT) {
       const int x = blockIdx.x * kBlock + i;
-      if (x < a.pages && a.refs_out[x] == 0) ++v;
+      if (x < a.pages && a.held[x] == 0) ++v;
     }
-    v = block_sum(v);
+    v = block_sum<kT>(v);
     if (threadIdx.x == 0) a.counts[blockIdx.x] = v;
     return;
   }
-  const int s = ((int)blockIdx.x - a.blocks) * kT + threadIdx.x;
-  if (s >= a.n) return;
-  const Row r = row_of(a, s, parent_of(a, s));
-  if (r.page >= 0 && a.refs_out[r.page] > 1) {
-    atomicAdd(a.growing + r.page, 1);
-    atomicMax(a.highest + r.page, s);
-  }
-}
-
-// sum of counts[0 .. n)
-__device__ __forceinline__ int sum_counts(const int* counts, int n) {
-  int v = 0;
-  for (int i = threadIdx.x; i < n; i += kT) v += counts[i];
-  return block_sum(v);
-}
-
-// workgroup `blocks` numbers the rows' requests, the others list their block's free pages
-__global__ __launch_bounds__(kT) void update_rank(Upd a) {
-  if ((int)blockIdx.x < a.blocks) {
-    int before = sum_counts(a.counts, blockIdx.x);
-    for (int i = 0; i < kBlock; i += kT) {
-      const int x = blockIdx.x * kBlock + i + threadIdx.x;
-      const bool free = x < a.pages && a.refs_out[x] == 0;
-      int total;
-      const int k = block_scan(free, total);
-      if (free) a.pool[before + k] = x;
-      before += total;
-    }
-    return;
-  }
-  long long asked = 0;  // (n * width < 2^31 is not given: more than `pages` is all that matters)
+  long long asked = 0;
   for (int s0 = 0; s0 < a.n; s0 += kT) {
     const int s = s0 + threadIdx.x;
     int need = 0, cow = 0;
     if (s < a.n) {
       const Row r = row_of(a, s, parent_of(a, s));
-      if (r.page >= 0) {
-        const int refs = a.refs_out[r.page];
-        cow = refs > 1 && !(a.growing[r.page] == refs && a.highest[r.page] == s);
-      }
+      cow = r.page >= 0 && takes_copy(a.held[r.page], a.growing[r.page], a.highest[r.page], s);
       need = pages_of(r.total, a.sh) - r.kept + cow;
       a.cow[s] = cow;
     }
-    int total;
-    const int k = block_scan(need, total);
-    if (s < a.n) a.first[s] = (int)min(asked + k, (long long)INT32_MAX);
+    long long total;
+    const long long k = block_scan<kT>((long long)need, total);
+    if (s < a.n) a.first[s] = clamp_sum(asked + k);
     asked += total;
   }
-  if (threadIdx.x == 0) a.first[a.n] = (int)min(asked, (long long)INT32_MAX);
+  if (threadIdx.x == 0) a.first[a.n] = clamp_sum(asked);
 }
 
-__device__ __forceinline__ void copy16(unsigned char* dst, const unsigned char* src) {
-  *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-}
-
-// grid: x = column blocks, y = rows: the table; then every workgroup takes its share of the copies
+// workgroups 0 .. blocks-1: the reference counts of their pages; the others: rows, then shares of the copies
 __global__ __launch_bounds__(kT) void update_commit(Upd a) {
-  const int free = sum_counts(a.counts, a.blocks);
+  __shared__ int s_block, s_before;
+  const int tid = threadIdx.x;
+  int v = 0, below = 0;
+  for (int i = tid; i < a.blocks; i += kT) {
+    v += a.counts[i];
+    if (i < (int)blockIdx.x) below += a.counts[i];
+  }
+  const int free = block_sum<kT>(v);
   const int asked = a.first[a.n];
   const bool ok = asked <= free;
-  const int wg = blockIdx.y * gridDim.x + blockIdx.x, wgs = gridDim.x * gridDim.y;
-  if (wg == 0 && threadIdx.x == 0) a.short_out[0] = ok ? 0 : asked - free;
+  if (blockIdx.x == 0 && tid == 0) a.short_out[0] = ok ? 0 : asked - free;
   if (!ok) {
-    // the state as it was
-    for (long long e = (long long)wg * kT + threadIdx.x; e < (long long)a.n * a.width; e += (long long)wgs * kT)
-      a.table_out[e] = a.table[e];
-    for (int e = wg * kT + threadIdx.x; e < a.pages; e += wgs * kT) a.refs_out[e] = a.refs[e];
-    for (int e = wg * kT + threadIdx.x; e < a.n; e += wgs * kT) a.lens_out[e] = a.lens[e];
+    keep_state(a, blockIdx.x, gridDim.x, kT);
     return;
   }
-  const int c = blockIdx.x * kT + threadIdx.x;
-  for (int s = blockIdx.y; s < a.n; s += gridDim.y) {
+  if ((int)blockIdx.x < a.blocks) {
+    int before = block_sum<kT>(below);  // free pages of the blocks before
+    for (int i = 0; i < kBlock; i += kT) {
+      const int x = blockIdx.x * kBlock + i + tid;
+      const int held = x < a.pages ? a.held[x] : 1;
+      int total;
+      const int k = before + block_scan<kT>((int)(held == 0), total);
+      before += total;
+      if (x >= a.pages) continue;
+      a.refs_out[x] = held == 0 ? (k < asked ? 1 : 0) : held - copies_of(held, a.growing[x]);
+    }
+    return;
+  }
+  const int wg = blockIdx.x - a.blocks, wgs = gridDim.x - a.blocks;
+  for (int s = wg; s < a.n; s += wgs) {
     const int p = parent_of(a, s);
     const Row r = row_of(a, s, p);
-    const int cow = a.cow[s], first = a.first[s];
-    if (c == 0) {
-      a.lens_out[s] = r.total;
-      if (cow) atomicSub(a.refs_out + r.page, 1);
+    const int cow = a.cow[s], first = a.first[s], need = a.first[s + 1] - first;
+    const int total = pages_of(r.total, a.sh);
+    int* out = a.table_out + (long long)s * a.width;
+    if (tid == 0) a.lens_out[s] = r.total;
+    for (int c = tid; c < a.width; c += kT) {
+      if (c < r.kept - cow) {
+        const int x = a.table[(long long)p * a.width + c];
+        out[c] = (unsigned)x < (unsigned)a.pages ? x : -1;
+      } else if (c >= total) {
+        out[c] = -1;
+      }
     }
-    if (c >= a.width) continue;
-    int x = -1;
-    if (c < r.kept) {
-      x = a.table[(long long)p * a.width + c];
-      if ((unsigned)x >= (unsigned)a.pages) x = -1;
-      if (cow && c == r.kept - 1) x = -2;
-    } else if (c < pages_of(r.total, a.sh)) {
-      x = -3;
+    if (need == 0) continue;
+    // the row's free pages, first .. first + need - 1 in rank, to the columns from kept - cow on: the block that
+    // holds the first by the blocks' counts, then block by block
+    int before = 0;
+    for (int b0 = 0; b0 < a.blocks; b0 += kT) {
+      const int here = b0 + tid < a.blocks ? a.counts[b0 + tid] : 0;
+      int sum;
+      const int k = before + block_scan<kT>(here, sum);
+      if (k <= first && first < k + here) s_block = b0 + tid, s_before = k;  // (one thread: first < free)
+      if (first < before + sum) break;
+      before += sum;
     }
-    if (x < -1) {
-      x = a.pool[first + (x == -2 ? 0 : cow + c - r.kept)];
-      a.refs_out[x] = 1;  // (asked for once, held by nothing else)
+    __syncthreads();
+    before = s_before;
+    for (int b = s_block; b < a.blocks && before < first + need; ++b) {
+      for (int i = 0; i < kBlock; i += kT) {
+        const int x = b * kBlock + i + tid;
+        const bool f = x < a.pages && a.held[x] == 0;
+        int sum;
+        const int k = before + block_scan<kT>((int)f, sum) - first;
+        before += sum;
+        if (f && k >= 0 && k < need) out[r.kept - cow + k] = x;
+      }
     }
-    a.table_out[(long long)s * a.width + c] = x;
-  }
-  if (!a.data) return;
-  const long long head_bytes = (long long)a.ps * a.rb, plane = head_bytes * a.heads * a.pages;
-  for (long long e = wg; e < (long long)a.n * a.planes; e += wgs) {
-    const int s = (int)(e / a.planes), pl = (int)(e % a.planes);
-    if (!a.cow[s]) continue;
-    const Row r = row_of(a, s, parent_of(a, s));
-    const int dst = a.pool[a.first[s]];
-    const int used = (r.keep & (a.ps - 1)) * a.rb / 16;  // 16-byte chunks a head
-    unsigned char* base = a.data + pl * plane;
-    for (int i = threadIdx.x; i < a.heads * used; i += kT) {
-      const long long off = (long long)(i / used) * head_bytes + (long long)(i % used) * 16;
-      copy16(base + dst * head_bytes * a.heads + off, base + r.page * head_bytes * a.heads + off);
-    }
+    if (!cow || !a.data) continue;
+    __syncthreads();  // (the row's own writes)
+    const int dst = out[r.kept - 1];
+    copy_used(a, 0, a.planes, r.page, dst, r.keep, tid, kT);
   }
 }
 
@@ -253,13 +381,20 @@ struct Cmp {
   int *counts, *rank, *src, *dst, *moved;  // workspace
 };
 
+// sum of counts[0 .. n)
+__device__ __forceinline__ int sum_counts(const int* counts, int n) {
+  int v = 0;
+  for (int i = threadIdx.x; i < n; i += kT) v += counts[i];
+  return block_sum<kT>(v);
+}
+
 __global__ __launch_bounds__(kT) void compact_count(Cmp a) {
   int v = 0;
   for (int i = threadIdx.x; i < kBlock; i += kT) {
     const int x = blockIdx.x * kBlock + i;
     if (x < a.pages && a.refs[x] > 0) ++v;
   }
-  v = block_sum(v);
+  v = block_sum<kT>(v);
   if (threadIdx.x == 0) a.counts[blockIdx.x] = v;
 }
 
@@ -269,13 +404,13 @@ __global__ __launch_bounds__(kT) void compact_rank(Cmp a) {
   const int lb = live / kBlock;
   int v = 0;
   for (int i = threadIdx.x; i < live - lb * kBlock; i += kT) v += a.refs[lb * kBlock + i] > 0;
-  const int below = sum_counts(a.counts, lb) + block_sum(v);
+  const int below = sum_counts(a.counts, lb) + block_sum<kT>(v);
   int before = sum_counts(a.counts, blockIdx.x);
   for (int i = 0; i < kBlock; i += kT) {
     const int x = blockIdx.x * kBlock + i + threadIdx.x;
     const bool on = x < a.pages && a.refs[x] > 0;
     int total;
-    const int k = before + block_scan(on, total);  // live pages before x
+    const int k = before + block_scan<kT>((int)on, total);  // live pages before x
     before += total;
     if (x >= a.pages) continue;
     if (on && x >= live) {
@@ -391,26 +526,28 @@ int mfl_pages_update(const int32_t* table, const int32_t* lens, const int32_t* r
   a.blocks = (int)((pages + kBlock - 1) / kBlock);
   a.table_out = table_out, a.lens_out = lens_out, a.refs_out = refs_out, a.short_out = short_out;
   char* ws = static_cast<char*>(workspace);
+  a.held = reinterpret_cast<int*>(ws), ws += pad16(pages);
   a.growing = reinterpret_cast<int*>(ws), ws += pad16(pages);
   a.highest = reinterpret_cast<int*>(ws), ws += pad16(pages);
-  a.pool = reinterpret_cast<int*>(ws), ws += pad16(pages);
   a.counts = reinterpret_cast<int*>(ws), ws += pad16(a.blocks);
   a.first = reinterpret_cast<int*>(ws), ws += pad16(n + 1);
   a.cow = reinterpret_cast<int*>(ws);
   a.data = static_cast<unsigned char*>(data);
   a.planes = (int)planes, a.heads = (int)heads, a.rb = (int)row_bytes;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (n <= kSmallT && pages <= kSmallPages && n * width <= kSmallEntries) {
+    // enough workgroups for the copies (4 a workgroup at a time)
+    const int64_t want = data ? (n * planes + 3) / 4 : 1;
+    const unsigned wgs = (unsigned)(want < 1 ? 1 : want > kSmallWgs ? kSmallWgs : want);
+    hipLaunchKernelGGL(update_small, dim3(wgs), dim3(kSmallT), (size_t)(pages > 0 ? pages : 1) * 12, st, a);
+    return launched(who) ? 0 : 1;
+  }
   const unsigned cols = (unsigned)((width + kT - 1) / kT > 0 ? (width + kT - 1) / kT : 1);
   const unsigned rows = (unsigned)(n < 1 ? 1 : n > 32768 ? 32768 : n);
   if (pages > 0) hipLaunchKernelGGL(update_start, dim3((unsigned)((pages + kT - 1) / kT)), dim3(kT), 0, st, a);
   if (n > 0) hipLaunchKernelGGL(update_refs, dim3(cols, rows), dim3(kT), 0, st, a);
-  if (a.blocks + n > 0)
-    hipLaunchKernelGGL(update_marks, dim3((unsigned)(a.blocks + (n + kT - 1) / kT)), dim3(kT), 0, st, a);
-  hipLaunchKernelGGL(update_rank, dim3((unsigned)a.blocks + 1), dim3(kT), 0, st, a);
-  // enough workgroups for the copies as well
-  unsigned gy = rows;
-  if (data && cols * gy < (unsigned)kCopyWgs) gy = (kCopyWgs + cols - 1) / cols;
-  hipLaunchKernelGGL(update_commit, dim3(cols, gy), dim3(kT), 0, st, a);
+  hipLaunchKernelGGL(update_count, dim3((unsigned)a.blocks + 1), dim3(kT), 0, st, a);
+  hipLaunchKernelGGL(update_commit, dim3((unsigned)a.blocks + rows), dim3(kT), 0, st, a);
   return launched(who) ? 0 : 1;
 }
 

@@ -22,6 +22,9 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 2, torch.float16: 3}
 _ARGS = struct.Struct("=11Q22qd")  # mfl_paged_attention_args
 
 
+_NO_STRIDES = (0, 0, 0, 0)
+
+
 def _error(who):
     raise RuntimeError(f"{who}: " + _native.load_library().mfl_paged_last_error().decode(errors="replace"))
 
@@ -70,34 +73,46 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, *, k=None, v=None, star
     16 bytes; float32 statistics.  No gradients.
     """
     who = "paged_attention"
-    tag = _DTYPES.get(q.dtype)
+    dt = q.dtype
+    tag = _DTYPES.get(dt)
     if tag is None:
-        raise TypeError(f"{who}: unsupported dtype {q.dtype}")
+        raise TypeError(f"{who}: unsupported dtype {dt}")
     packed = offsets is not None
-    if q.dim() != (3 if packed else 4):
+    shape = q.shape
+    if len(shape) != (3 if packed else 4):
         raise ValueError(f"{who}: q must be {'(total, heads, dim)' if packed else '(n, rows, heads, dim)'}; got "
-                         f"{tuple(q.shape)}")
-    if (k is None) != (v is None):
-        raise ValueError(f"{who}: k and v come together")
+                         f"{tuple(shape)}")
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
         raise ValueError(f"{who}: k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must be (pages, "
                          "kv_heads, page_size, dim)")
-    dt = q.dtype
+    if table.dim() != 2:
+        raise ValueError(f"{who}: table must be (n, width); got {tuple(table.shape)}")
+    n, width = table.shape
+    pages, kvh, ps, d = k_pages.shape
+    heads = shape[-2]
+    if shape[-1] != d or kvh < 1 or heads < 1 or heads % kvh:
+        raise ValueError(f"{who}: q heads x dim {tuple(shape[-2:])} do not fit pages {tuple(k_pages.shape)}")
+    if packed:
+        total = shape[0]
+        rows = total if max_rows is None else min(int(max_rows), total)
+        if rows < 0:
+            raise ValueError(f"{who}: max_rows {max_rows}")
+        offsets = _i32(who, "offsets", offsets, (n + 1,))
+    else:
+        total, rows = 0, shape[1]
+        if shape[0] != n:
+            raise ValueError(f"{who}: q has {shape[0]} sequences, table {n}")
+    if (k is None) != (v is None):
+        raise ValueError(f"{who}: k and v come together")
     if k_pages.dtype != dt or v_pages.dtype != dt or k is not None and (k.dtype != dt or v.dtype != dt):
         raise TypeError(f"{who}: pages, k and v must be {dt} like q; got {k_pages.dtype}, {v_pages.dtype}"
                         + ("" if k is None else f", {k.dtype}, {v.dtype}"))
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError(f"{who}: pages must be contiguous")
-    pages, kvh, ps, d = k_pages.shape
-    heads = q.shape[-2]
-    if q.shape[-1] != d or kvh < 1 or heads < 1 or heads % kvh:
-        raise ValueError(f"{who}: q heads x dim {tuple(q.shape[-2:])} do not fit pages {tuple(k_pages.shape)}")
-    if k is not None and (k.shape != q.shape[:-2] + (kvh, d) or v.shape != k.shape):
-        raise ValueError(f"{who}: k / v must be {tuple(q.shape[:-2]) + (kvh, d)}; got {tuple(k.shape)}, "
-                         f"{tuple(v.shape)}")
-    if table.dim() != 2:
-        raise ValueError(f"{who}: table must be (n, width); got {tuple(table.shape)}")
-    n, width = table.shape
+    if k is not None:
+        want = (total, kvh, d) if packed else (n, rows, kvh, d)
+        if k.shape != want or v.shape != want:
+            raise ValueError(f"{who}: k / v must be {want}; got {tuple(k.shape)}, {tuple(v.shape)}")
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad
                                     or k is not None and (k.requires_grad or v.requires_grad)):
         raise RuntimeError(f"{who}: inference only (no gradient); call it under torch.no_grad()")
@@ -105,39 +120,29 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, *, k=None, v=None, star
     kv_lens = _i32(who, "kv_lens", kv_lens, (n,))
     if starts is not None:
         starts = _i32(who, "starts", starts, (n,))
-    if packed:
-        offsets = _i32(who, "offsets", offsets, (n + 1,))
-        total = q.shape[0]
-        rows = total if max_rows is None else min(int(max_rows), total)
-    else:
-        if q.shape[0] != n:
-            raise ValueError(f"{who}: q has {q.shape[0]} sequences, table {n}")
-        total, rows = 0, q.shape[1]
-    if rows < 0:
-        raise ValueError(f"{who}: max_rows {max_rows}")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
-        raise ValueError(f"{who}: out must be a contiguous {tuple(q.shape)} {q.dtype} tensor")
+    if out is not None and (out.shape != shape or out.dtype != dt or not out.is_contiguous()):
+        raise ValueError(f"{who}: out must be a contiguous {tuple(shape)} {dt} tensor")
     dev = _native.device_index(who, (("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("k", k), ("v", v),
                                      ("table", table), ("kv_lens", kv_lens), ("starts", starts), ("offsets", offsets),
                                      ("out", out)))
+    q, qs = _rows16(q)
     zero_tail = packed and out is None
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    q, qs = _rows16(q)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dt, device=q.device)
     if k is None:
         kp = vp = 0
-        ks = vs = (0, 0, 0, 0)
+        ks = vs = _NO_STRIDES
     else:
         (k, ks), (v, vs) = _rows16(k), _rows16(v)
         kp, vp = k.data_ptr(), v.data_ptr()
     if packed:
         qs, ks, vs = (0,) + qs, (0,) + ks[-3:], (0,) + vs[-3:]
     capacity = width * ps
+    ptrs = (q.data_ptr(), kp, vp, k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr())
     fixed = (table.data_ptr(), kv_lens.data_ptr(), 0 if starts is None else starts.data_ptr(),
              offsets.data_ptr() if packed else 0, n, rows, total, heads, kvh, d, pages, ps, width,
              capacity if max_kv is None else min(int(max_kv), capacity), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
              vs[0], vs[1], vs[2], tag, 1 if causal else 0, 1 if zero_tail else 0, d ** -0.5 if scale is None else scale)
-    ptrs = (q.data_ptr(), kp, vp, k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr())
     lib = _native.load_library()
     args = _ARGS.pack(*ptrs, 0, *fixed)
     need = lib.mfl_paged_attention_workspace_bytes(args)
