@@ -5,7 +5,8 @@
 // token of the tile occurs in the row's history is counted in LDS (integer atomics: any order gives the same counts);
 // the first of a token's occurrences to be seen again then penalises its logit once and leaves it in LDS, so that
 // the dense pass only picks it up.  The row's history is read once per tile, out of the L2: long histories
-// take tiles of 8,192 tokens (1,024 threads), short ones tiles of 2,048, of which there are more to fill the chip.
+// take tiles of 8,192 tokens (1,024 threads), short ones tiles of 2,048, of which there are more to fill the chip;
+// a few rows of up to 16,384 tokens are one tile each, which needs no second launch.
 // The best token goes by 64-bit keys (the value's order-preserving bits above the complement of the index: ties go to
 // the lowest index, NaN above all).  Rows of one tile finish in the same launch, else logits_join merges the
 // tiles' (key, sum of exponentials) pairs.
@@ -28,6 +29,7 @@ namespace {
 constexpr int kV = 8;                 // tokens a thread
 constexpr int kFew = 256, kMany = 1024;  // threads a workgroup: short / long histories
 constexpr int kLongHistory = 512;
+constexpr int kFewRows = 512;         // rows of which one-tile workgroups are no more than two a CU
 constexpr int kTok = 4;               // tokens of the history a thread holds
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -173,14 +175,13 @@ __device__ __forceinline__ void finish(const Args& a, int row, const Stat& r) {
 
 constexpr uint32_t kNone = 0xffffffffu;  // no penalised value (a NaN that the penalties never make)
 
-template <class T, class O, int THREADS>
-__global__ __launch_bounds__(THREADS) void logits_tile(Args a) {
-  constexpr int kTile = THREADS * kV;
+template <class T, class O, int THREADS, int NCH>
+__global__ __launch_bounds__(THREADS, NCH == 1 ? 8 : 4) void logits_tile(Args a) {
+  constexpr int kPass = THREADS * kV, kTile = kPass * NCH;
   __shared__ __attribute__((aligned(16))) uint32_t value[kTile];  // penalised logits
   __shared__ __attribute__((aligned(16))) uint32_t count[kTile];
   const int row = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
   const int v0 = tile * kTile, nv = min(kTile, a.vocab - v0);
-  const int i = threadIdx.x * kV, m = max(0, min(kV, nv - i));
   const T* src = reinterpret_cast<const T*>(a.logits) + row * a.logits_row + v0;
   // the history's first kTok tokens a thread stay in registers, fetched with the logits
   const int len = a.hist == 0 ? 0 : a.token_lens ? max(0, min(a.token_lens[row], a.hist)) : a.hist;
@@ -191,41 +192,51 @@ __global__ __launch_bounds__(THREADS) void logits_tile(Args a) {
     const int j = t * THREADS + (int)threadIdx.x;
     held[t] = j < len ? tok[j] : -1;
   }
-  float x[kV], b[kV];
-  uint32_t ok = 0xffu;
-  if (m > 0) {
-    load8(src + i, m, x);
-    if (a.bias) load8(a.bias + row * a.bias_row + v0 + i, m, b);
-    if (a.kind) {
-      const int mr = a.states ? a.states[row] : (a.allowed_rows == 1 ? 0 : row);  // mask row
-      if ((unsigned)mr < (unsigned)a.allowed_rows) {
-        if (a.kind == 2) {
-          // (v0 and i are multiples of 8: the eight bits are one byte of a word)
-          ok = a.allowed[(long long)mr * a.allowed_row * 4 + (v0 + i) / 8];
-        } else {
-          const unsigned char* p = a.allowed + (long long)mr * a.allowed_row + v0 + i;
-          unsigned long long w = 0;
-          if (m == kV) {
-            __builtin_memcpy(&w, p, 8);
-          } else {
+  int mr = -1;  // mask row
+  if (a.kind) {
+    mr = a.states ? a.states[row] : (a.allowed_rows == 1 ? 0 : row);
+    if ((unsigned)mr >= (unsigned)a.allowed_rows) mr = -1;
+  }
+  float x[NCH][kV], b[NCH][kV];  // everything the row needs is fetched before the history is counted
+  uint32_t ok[NCH];
 #pragma unroll
-            for (int e = 0; e < kV; ++e)
-              if (e < m) w |= (unsigned long long)p[e] << (8 * e);
-          }
-          ok = 0;
+  for (int c = 0; c < NCH; ++c) {
+    const int i = c * kPass + (int)threadIdx.x * kV, m = max(0, min(kV, nv - i));
+    ok[c] = 0xffu;
+    if (m == 0) continue;
+    load8(src + i, m, x[c]);
+    if (a.bias) load8(a.bias + row * a.bias_row + v0 + i, m, b[c]);
+    if (mr < 0) continue;
+    if (a.kind == 2) {
+      // (v0 and i are multiples of 8: the eight bits are one byte of a word)
+      ok[c] = a.allowed[(long long)mr * a.allowed_row * 4 + (v0 + i) / 8];
+    } else {
+      const unsigned char* p = a.allowed + (long long)mr * a.allowed_row + v0 + i;
+      unsigned long long w = 0;
+      if (m == kV) {
+        __builtin_memcpy(&w, p, 8);
+      } else {
 #pragma unroll
-          for (int e = 0; e < kV; ++e) ok |= ((w >> (8 * e)) & 0xffu ? 1u : 0u) << e;
-        }
+        for (int e = 0; e < kV; ++e)
+          if (e < m) w |= (unsigned long long)p[e] << (8 * e);
       }
+      ok[c] = 0;
+#pragma unroll
+      for (int e = 0; e < kV; ++e) ok[c] |= ((w >> (8 * e)) & 0xffu ? 1u : 0u) << e;
     }
   }
   bool any = false;
   if (len > 0) {
     const uint4 none = {kNone, kNone, kNone, kNone}, zero = {0, 0, 0, 0};
-    uint4* vp = reinterpret_cast<uint4*>(value + i);
-    uint4* cp = reinterpret_cast<uint4*>(count + i);
-    vp[0] = none, vp[1] = none;
-    cp[0] = zero, cp[1] = zero;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int i = c * kPass + (int)threadIdx.x * kV;
+      if (i >= nv) continue;
+      uint4* vp = reinterpret_cast<uint4*>(value + i);
+      uint4* cp = reinterpret_cast<uint4*>(count + i);
+      vp[0] = none, vp[1] = none;
+      cp[0] = zero, cp[1] = zero;
+    }
     __syncthreads();
     const auto add = [&](int v) {
       if ((unsigned)v < (unsigned)nv) {
@@ -257,27 +268,39 @@ __global__ __launch_bounds__(THREADS) void logits_tile(Args a) {
     }
   }
   const bool stats = a.best || a.lse || a.logprob;
-  if (m > 0) {
-    if (any) {
+  Stat t{0ull, -INFINITY, 0.f};
 #pragma unroll
-      for (int e = 0; e < kV; ++e) {
-        const uint32_t y = value[i + e];
-        x[e] = y == kNone ? x[e] : __uint_as_float(y);
+  for (int c = 0; c < NCH; ++c) {
+    const int i = c * kPass + (int)threadIdx.x * kV, m = max(0, min(kV, nv - i));
+    if (m > 0) {
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+          const uint32_t y = value[i + e];
+          x[c][e] = y == kNone ? x[c][e] : __uint_as_float(y);
+        }
       }
+      if (a.bias) {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) x[c][e] = x[c][e] + b[c][e];
+      }
+#pragma unroll
+      for (int e = 0; e < kV; ++e) x[c][e] = (ok[c] >> e) & 1u ? x[c][e] : -INFINITY;
+      if (a.out) store8(reinterpret_cast<O*>(a.out) + row * a.out_row + v0 + i, m, x[c]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kV; ++e) x[c][e] = -INFINITY;
     }
-    if (a.bias) {
-#pragma unroll
-      for (int e = 0; e < kV; ++e) x[e] = x[e] + b[e];
+    if (stats) {
+      const Stat u = wave_stat(x[c], m, v0 + i);
+      if (NCH == 1)
+        t = u;
+      else
+        merge(t, u.key, u.m, u.s);
     }
-#pragma unroll
-    for (int e = 0; e < kV; ++e) x[e] = (ok >> e) & 1u ? x[e] : -INFINITY;
-    if (a.out) store8(reinterpret_cast<O*>(a.out) + row * a.out_row + v0 + i, m, x);
-  } else {
-#pragma unroll
-    for (int e = 0; e < kV; ++e) x[e] = -INFINITY;
   }
   if (!stats) return;
-  const Stat r = block_stat<THREADS>(wave_stat(x, m, v0 + i));
+  const Stat r = block_stat<THREADS>(t);
   if (threadIdx.x != 0) return;
   if (a.tiles == 1) {
     finish(a, row, r);
@@ -322,12 +345,22 @@ bool bad(const char* fmt, ...) {
 
 int esize(int64_t t) { return t == 0 ? 4 : t == 2 || t == 3 ? 2 : 0; }
 
-int threads_of(const mfl_logits_args* p) { return p->hist > kLongHistory ? kMany : kFew; }
+struct Plan {
+  int threads, passes, tiles;
+};
 
-int tiles_of(const mfl_logits_args* p) {
-  const int64_t tile = (int64_t)threads_of(p) * kV;
-  return (int)((p->vocab + tile - 1) / tile);
+Plan plan_of(const mfl_logits_args* p) {
+  Plan r{p->hist > kLongHistory ? kMany : kFew, 1, 0};
+  if (p->n <= kFewRows && p->vocab <= 2 * kMany * kV) {
+    r.threads = p->vocab <= kFew * kV ? kFew : kMany;
+    r.passes = p->vocab <= kMany * kV ? 1 : 2;
+  }
+  const int64_t tile = (int64_t)r.threads * r.passes * kV;
+  r.tiles = (int)((p->vocab + tile - 1) / tile);
+  return r;
 }
+
+int tiles_of(const mfl_logits_args* p) { return plan_of(p).tiles; }
 
 bool check(const mfl_logits_args* p) {
   const char* who = "mfl_logits_process";
@@ -352,22 +385,24 @@ bool check(const mfl_logits_args* p) {
 }
 
 template <class T, class O>
-void launch_out(const Args& a, int threads, hipStream_t st) {
+void launch_out(const Args& a, const Plan& pl, hipStream_t st) {
   const dim3 grid((unsigned)a.n * (unsigned)a.tiles);
-  if (threads == kMany)
-    hipLaunchKernelGGL((logits_tile<T, O, kMany>), grid, dim3(kMany), 0, st, a);
+  if (pl.passes == 2)
+    hipLaunchKernelGGL((logits_tile<T, O, kMany, 2>), grid, dim3(kMany), 0, st, a);
+  else if (pl.threads == kMany)
+    hipLaunchKernelGGL((logits_tile<T, O, kMany, 1>), grid, dim3(kMany), 0, st, a);
   else
-    hipLaunchKernelGGL((logits_tile<T, O, kFew>), grid, dim3(kFew), 0, st, a);
+    hipLaunchKernelGGL((logits_tile<T, O, kFew, 1>), grid, dim3(kFew), 0, st, a);
 }
 
 template <class T>
-void launch(const Args& a, int64_t out_dtype, int threads, hipStream_t st) {
+void launch(const Args& a, int64_t out_dtype, const Plan& pl, hipStream_t st) {
   if (out_dtype == 0)
-    launch_out<T, float>(a, threads, st);
+    launch_out<T, float>(a, pl, st);
   else if (out_dtype == 2)
-    launch_out<T, __bf16>(a, threads, st);
+    launch_out<T, __bf16>(a, pl, st);
   else
-    launch_out<T, _Float16>(a, threads, st);
+    launch_out<T, _Float16>(a, pl, st);
 }
 
 }  // namespace
@@ -419,11 +454,11 @@ int mfl_logits_process(const mfl_logits_args* p, void* stream) {
   a.rep_s = (float)p->repetition, a.pres_s = (float)p->presence, a.freq_s = (float)p->frequency;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (p->dtype == 0)
-    launch<float>(a, p->out_dtype, threads_of(p), st);
+    launch<float>(a, p->out_dtype, plan_of(p), st);
   else if (p->dtype == 2)
-    launch<__bf16>(a, p->out_dtype, threads_of(p), st);
+    launch<__bf16>(a, p->out_dtype, plan_of(p), st);
   else
-    launch<_Float16>(a, p->out_dtype, threads_of(p), st);
+    launch<_Float16>(a, p->out_dtype, plan_of(p), st);
   if (tiles > 1 && stats) hipLaunchKernelGGL(logits_join, dim3((unsigned)a.n), dim3(64), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {

@@ -30,6 +30,29 @@ def _penalty(who, name, x, n, default):
     return None, x
 
 
+def _rows_i32(who, name, t, n):
+    if t.dtype != torch.int32 or t.shape != (n,):
+        raise ValueError(f"{who}: {name} must be ({n},) int32")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _mask(who, allowed, states, n, vocab):
+    """(mask, kind, mask rows, elements a row)"""
+    if allowed.dtype in (torch.bool, torch.uint8):
+        kind, cols = 1, vocab
+    elif allowed.dtype == torch.int32:
+        kind, cols = 2, (vocab + 31) // 32
+    else:
+        raise TypeError(f"{who}: allowed must be bool (a token an element) or int32 (32 tokens an element), got "
+                        f"{allowed.dtype}")
+    if allowed.dim() not in (1, 2) or allowed.shape[-1] != cols:
+        raise ValueError(f"{who}: allowed must be ({cols},) or (rows, {cols}); got {tuple(allowed.shape)}")
+    rows = 1 if allowed.dim() == 1 else allowed.shape[0]
+    if rows < 1 or (states is None and rows not in (1, n)):
+        raise ValueError(f"{who}: {rows} mask rows for {n} rows of logits without states")
+    return allowed if allowed.is_contiguous() else allowed.contiguous(), kind, rows, cols
+
+
 def _run(who, logits, tokens, token_lens, repetition, presence, frequency, bias, allowed, states, out, write, stats):
     tag = _DTYPES.get(logits.dtype)
     if tag is None:
@@ -39,21 +62,22 @@ def _run(who, logits, tokens, token_lens, repetition, presence, frequency, bias,
     n, vocab = logits.shape
     if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError(f"{who}: inference only (no gradient); call it under torch.no_grad()")
-    hist = 0
+    hist = tokens_row = 0
     if tokens is not None:
         if tokens.dim() != 2 or tokens.shape[0] != n:
             raise ValueError(f"{who}: tokens must be ({n}, length); got {tuple(tokens.shape)}")
         if tokens.dtype != torch.int32:
             raise TypeError(f"{who}: tokens must be int32, got {tokens.dtype}")
         hist = tokens.shape[1]
-        if hist and tokens.stride(1) != 1:
-            tokens = tokens.contiguous()
-    if token_lens is not None:
-        if tokens is None:
-            raise ValueError(f"{who}: token_lens without tokens")
-        if token_lens.dtype != torch.int32 or tuple(token_lens.shape) != (n,):
-            raise ValueError(f"{who}: token_lens must be ({n},) int32")
-        token_lens = token_lens.contiguous()
+        if hist:
+            tokens_row, step = tokens.stride()
+            if step != 1:
+                tokens = tokens.contiguous()
+                tokens_row = hist
+        if token_lens is not None:
+            token_lens = _rows_i32(who, "token_lens", token_lens, n)
+    elif token_lens is not None:
+        raise ValueError(f"{who}: token_lens without tokens")
     rep_t, rep = _penalty(who, "repetition", repetition, n, 1.0)
     pres_t, pres = _penalty(who, "presence", presence, n, 0.0)
     freq_t, freq = _penalty(who, "frequency", frequency, n, 0.0)
@@ -61,36 +85,19 @@ def _run(who, logits, tokens, token_lens, repetition, presence, frequency, bias,
     if bias is not None:
         if bias.dtype != torch.float32:
             raise TypeError(f"{who}: bias must be float32, got {bias.dtype}")
-        if tuple(bias.shape) not in ((vocab,), (n, vocab)):
+        if bias.shape != (vocab,) and bias.shape != (n, vocab):
             raise ValueError(f"{who}: bias must be ({vocab},) or ({n}, {vocab}); got {tuple(bias.shape)}")
         if bias.stride(-1) != 1 and vocab > 1:
             bias = bias.contiguous()
         bias_row = bias.stride(0) if bias.dim() == 2 else 0
     kind = mask_rows = mask_row = 0
     if allowed is not None:
-        if allowed.dtype in (torch.bool, torch.uint8):
-            kind, cols = 1, vocab
-        elif allowed.dtype == torch.int32:
-            kind, cols = 2, (vocab + 31) // 32
-        else:
-            raise TypeError(f"{who}: allowed must be bool (a token an element) or int32 (32 tokens an element), got "
-                            f"{allowed.dtype}")
-        if allowed.dim() not in (1, 2) or allowed.shape[-1] != cols:
-            raise ValueError(f"{who}: allowed must be ({cols},) or (rows, {cols}); got {tuple(allowed.shape)}")
-        allowed = allowed.view(1, cols) if allowed.dim() == 1 else allowed
-        mask_rows = allowed.shape[0]
-        if mask_rows < 1 or (states is None and mask_rows not in (1, n)):
-            raise ValueError(f"{who}: {mask_rows} mask rows for {n} rows of logits without states")
-        allowed = allowed.contiguous()
-        mask_row = cols
-    if states is not None:
-        if allowed is None:
-            raise ValueError(f"{who}: states without allowed")
-        if states.dtype != torch.int32 or tuple(states.shape) != (n,):
-            raise ValueError(f"{who}: states must be ({n},) int32")
-        states = states.contiguous()
-    if out is not None and (tuple(out.shape) != (n, vocab) or out.dtype not in _DTYPES or
-                            (vocab > 1 and out.stride(1) != 1)):
+        allowed, kind, mask_rows, mask_row = _mask(who, allowed, states, n, vocab)
+        if states is not None:
+            states = _rows_i32(who, "states", states, n)
+    elif states is not None:
+        raise ValueError(f"{who}: states without allowed")
+    if out is not None and (out.shape != (n, vocab) or out.dtype not in _DTYPES or (vocab > 1 and out.stride(1) != 1)):
         raise ValueError(f"{who}: out must be ({n}, {vocab}) with contiguous rows, float32, bfloat16 or float16")
     dev = _native.device_index(who, (("logits", logits), ("tokens", tokens), ("token_lens", token_lens),
                                      ("repetition", rep_t), ("presence", pres_t), ("frequency", freq_t), ("bias", bias),
@@ -99,24 +106,26 @@ def _run(who, logits, tokens, token_lens, repetition, presence, frequency, bias,
         logits = logits.contiguous()
     lib = _native.load_library()
     with _native.on_device(dev):
+        device = logits.device
         if write and out is None:
-            out = torch.empty(n, vocab, dtype=torch.float32, device=logits.device)
-        best = torch.empty(n, dtype=torch.int64, device=logits.device) if stats else None
-        rest = torch.empty(n, dtype=torch.float32, device=logits.device) if stats else None
-
-        def ptr(t):
-            return 0 if t is None else t.data_ptr()
-
-        head = (logits.data_ptr(), ptr(out), ptr(best), ptr(rest) if write else 0, 0 if write else ptr(rest),
-                ptr(tokens) if hist else 0, ptr(token_lens), ptr(rep_t), ptr(pres_t), ptr(freq_t), ptr(bias), ptr(allowed),
-                ptr(states))
-        tail = (n, vocab, tag, _DTYPES[out.dtype] if out is not None else 0, logits.stride(0),
-                out.stride(0) if out is not None else 0, hist, tokens.stride(0) if hist else 0, bias_row, kind, mask_row,
-                mask_rows, rep, pres, freq)
+            out = torch.empty(n, vocab, dtype=torch.float32, device=device)
+        best = rest = None
+        bp = rp = 0
+        if stats:
+            best = torch.empty(n, dtype=torch.int64, device=device)
+            rest = torch.empty(n, dtype=torch.float32, device=device)
+            bp, rp = best.data_ptr(), rest.data_ptr()
+        head = (logits.data_ptr(), 0 if out is None else out.data_ptr(), bp, rp if write else 0, 0 if write else rp,
+                tokens.data_ptr() if hist else 0, 0 if token_lens is None else token_lens.data_ptr(),
+                0 if rep_t is None else rep_t.data_ptr(), 0 if pres_t is None else pres_t.data_ptr(),
+                0 if freq_t is None else freq_t.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                0 if allowed is None else allowed.data_ptr(), 0 if states is None else states.data_ptr())
+        tail = (n, vocab, tag, 0 if out is None else _DTYPES[out.dtype], logits.stride(0),
+                0 if out is None else out.stride(0), hist, tokens_row, bias_row, kind, mask_row, mask_rows, rep, pres, freq)
         args = _ARGS.pack(*head, 0, *tail)
         need = lib.mfl_logits_workspace_bytes(args)
         if need > 0:
-            ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+            ws = torch.empty(need, dtype=torch.uint8, device=device)
             args = _ARGS.pack(*head, ws.data_ptr(), *tail)
         if need < 0 or lib.mfl_logits_process(args, _native.raw_stream(dev)) != 0:
             raise RuntimeError(f"{who}: " + lib.mfl_logits_last_error().decode(errors="replace"))
