@@ -696,6 +696,11 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_att_split(Args a) {
 #pragma unroll
   for (int t = 0; t < NS; ++t)
     if (w0 + t < w1) issue(w0 + t);
+  if (a.kn && split == 0) {  // (while the first tiles fly)
+    // the tile writes the tokens whose first row it holds
+    const int i0 = (m0 + a.G - 1) / a.G, i1 = min(q.rows, (m0 + kRowsW + a.G - 1) / a.G);
+    write_chunk<T>(a, q, s, kn, vn, kh, i0, i1, threadIdx.x, 64 * NW);
+  }
   Cols<T, DP> w;
   cols_init<T, DP>(w, a, q, qb, kh, m0, lane);
   bool odd = false;  // a value that is not finite was scrubbed
@@ -722,11 +727,6 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_att_split(Args a) {
   if (__any(odd))
     add_non_finite<T, DP>(w, a, q, kn, vn, tab, kh, max(w0, least / kKeys) * kKeys, min(most, w1 * kKeys), lane);
   cols_sum<T, DP>(w);
-  if (a.kn && split == 0) {
-    // the tile writes the tokens whose first row it holds
-    const int i0 = (m0 + a.G - 1) / a.G, i1 = min(q.rows, (m0 + kRowsW + a.G - 1) / a.G);
-    write_chunk<T>(a, q, s, kn, vn, kh, i0, i1, threadIdx.x, 64 * NW);
-  }
   if constexpr (NW > 1) {
     __syncthreads();  // (every wave is done with its images)
     if (lane < 32) {
@@ -883,6 +883,10 @@ __global__ __launch_bounds__(64 * kWavesR, 2) void paged_att_rows(Args a) {
   };
   if (t0 < t1) issue(t0);
   if (t0 + 1 < t1) issue(t0 + 1);
+  if (a.kn && split == 0) {
+    const int i0 = (g0 + a.G - 1) / a.G, i1 = min(q.rows, (g0 + kTileR + a.G - 1) / a.G);
+    write_chunk<T>(a, q, s, kn, vn, kh, i0, i1, tid, 64 * kWavesR);
+  }
   Cols<T, DP> w;
   cols_init<T, DP>(w, a, q, qb, kh, m0, lane);
   bool odd = false;  // a value that is not finite was scrubbed
@@ -919,10 +923,6 @@ __global__ __launch_bounds__(64 * kWavesR, 2) void paged_att_rows(Args a) {
   if (least < most && __syncthreads_or(odd))
     add_non_finite<T, DP>(w, a, q, kn, vn, tab, kh, max(t0, least / kStep) * kStep, min(most, t1 * kStep), lane);
   cols_sum<T, DP>(w);
-  if (a.kn && split == 0) {
-    const int i0 = (g0 + a.G - 1) / a.G, i1 = min(q.rows, (g0 + kTileR + a.G - 1) / a.G);
-    write_chunk<T>(a, q, s, kn, vn, kh, i0, i1, tid, 64 * kWavesR);
-  }
   if (rg.used > 1) {
     cols_part<T, DP>(w, a, q, s, kh, m0, split, rg.used, lane);
   } else {
@@ -944,7 +944,7 @@ Plan plan_of(const mfl_paged_attention_args* p) {
   const int64_t rows = r.rows_kernel ? kTileR : kRowsW, step = r.rows_kernel ? 2 * kKeys : kKeys;
   r.tiles = (int)((M + rows - 1) / rows);
   if (r.tiles < 1) r.tiles = 1;
-  r.waves = r.rows_kernel ? kWavesR : kv <= 2 * kKeys ? 1 : 2;
+  r.waves = r.rows_kernel ? kWavesR : kv > 2 * kKeys && kv <= 512 ? 2 : 1;
   // tiles that there are: packed sequences share p->total rows
   int64_t base = p->n * r.tiles;
   if (p->offsets) {
@@ -953,13 +953,14 @@ Plan plan_of(const mfl_paged_attention_args* p) {
   }
   base *= p->kv_heads;
   if (base < 1) base = 1;
-  const int64_t least = r.rows_kernel ? 512 : 256;  // keys worth a range of their own
-  int64_t range = kv / ((1024 + base - 1) / base);
+  // the split kernel reaches the memory's rate with some 8,192 ranges of one wave each, of at least 256 keys; up to
+  // 512 keys two waves share a range instead, which needs no join
+  const int64_t least = r.rows_kernel ? 512 : kv <= 512 ? 512 : 256, want = r.rows_kernel ? 1024 : 8192;
+  int64_t range = kv / ((want + base - 1) / base);
   if (range < least) range = least;
   range = (range + step - 1) / step * step;
   int64_t sp = (kv + range - 1) / range;
   if (sp > 512) sp = 512;
-  if (r.waves == 1) sp = 1;
   r.splits = (int)sp;
   r.range = (int)range;
   return r;
