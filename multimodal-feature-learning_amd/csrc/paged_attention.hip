@@ -588,42 +588,77 @@ __device__ __forceinline__ void mark_rows(const Args& a, long long first, long l
     reinterpret_cast<int*>(a.ws)[e] = 0;
 }
 
-// what a workgroup has to do, the same in both kernels.  Work items are numbered ((s * tiles + tile) * splits +
-// split) * kvh + kh: the workgroups that read one key head's pages are kvh apart and, with 8 XCDs taking
-// workgroups in turn, share an L2 when kvh is a multiple of 8 (and a half or a quarter of them when it is 4 or 2)
+// what a workgroup has to do, the same in both kernels.  Work items are numbered (tile * splits + split) * kvh +
+// kh: the workgroups that read one key head's pages are kvh apart and, with 8 XCDs taking workgroups in
+// turn, share an L2 when kvh is a multiple of 8 (and a half or a quarter of them when it is 4 or 2).  Tiles: a.tiles
+// of each sequence, or (packed) those that the sequences have, counted here, and one or more behind the last (s == n)
 struct Job {
   int s, tile, split, kh;
+  int part, parts;  // of the workgroups of sequence s (or behind the last)
 };
-__device__ __forceinline__ Job job_of(const Args& a) {
+template <int ROWS>
+__device__ __forceinline__ Job job_of(const Args& a, int lane) {
   Job j;
   unsigned x = blockIdx.x;
   j.kh = x % (unsigned)a.kvh;
   x /= (unsigned)a.kvh;
   j.split = x % (unsigned)a.splits;
-  x /= (unsigned)a.splits;
-  j.tile = a.tiles - 1 - x % (unsigned)a.tiles;  // (a sequence's last rows see the most keys: they begin first)
-  j.s = x / (unsigned)a.tiles;
+  const int e = x / (unsigned)a.splits;
+  int mine = a.tiles, at;
+  if (!a.offsets) {
+    at = e % a.tiles;
+    j.s = e / a.tiles;
+  } else {
+    int before = 0;
+    j.s = a.n;
+    for (int c = 0; c < a.n; c += 64) {
+      const int i = min(a.n - 1, c + lane);
+      const long long o0 = max(0ll, min((long long)a.offsets[i], a.total));
+      const long long o1 = max(o0, min((long long)a.offsets[i + 1], a.total));
+      const int t = c + lane < a.n ? (min((int)(o1 - o0), a.rows) * a.G + ROWS - 1) / ROWS : 0;
+      int inc = t;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(inc, o);
+        if (lane >= o) inc += u;
+      }
+      const unsigned long long hit = __ballot(before + inc > e);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        j.s = c + l;
+        mine = __builtin_amdgcn_readlane(t, l);
+        at = e - before - (__builtin_amdgcn_readlane(inc, l) - mine);
+        break;
+      }
+      before += __builtin_amdgcn_readlane(inc, 63);
+    }
+    if (j.s == a.n) {
+      at = e - before;
+      mine = a.tiles - before;  // (a.tiles: one more than the sequences can have)
+    }
+  }
+  j.tile = j.s < a.n ? mine - 1 - at : 0;  // (a sequence's last rows see the most keys: they begin first)
+  j.part = (at * a.splits + j.split) * a.kvh + j.kh;
+  j.parts = mine * a.splits * a.kvh;
   return j;
 }
 
 // packed calls (s == n): the rows before the first sequence and behind the last
 __device__ __forceinline__ void rest_of_rows(const Args& a, const Job& j, int eb) {
-  const int part = (j.tile * a.splits + j.split) * a.kvh + j.kh, parts = a.tiles * a.splits * a.kvh;
   const long long r0 = max(0ll, min((long long)a.offsets[0], a.total));
   const long long r1 = max(r0, min((long long)a.offsets[a.n], a.total));
   if (a.zero_tail) {
-    zero_rows(a, 0, r0, part, parts, eb);
-    zero_rows(a, r1, a.total, part, parts, eb);
+    zero_rows(a, 0, r0, j.part, j.parts, eb);
+    zero_rows(a, r1, a.total, j.part, j.parts, eb);
   }
   if (a.splits > 1) {
-    mark_rows(a, 0, r0, part, parts);
-    mark_rows(a, r1, a.total, part, parts);
+    mark_rows(a, 0, r0, j.part, j.parts);
+    mark_rows(a, r1, a.total, j.part, j.parts);
   }
 }
 // ... and a sequence's rows behind its first a.rows
 __device__ __forceinline__ void rows_behind(const Args& a, const Job& j, const Seq& q) {
-  if (a.splits > 1 && a.offsets && q.q1 > q.q0 + q.rows)
-    mark_rows(a, q.q0 + q.rows, q.q1, (j.tile * a.splits + j.split) * a.kvh + j.kh, a.tiles * a.splits * a.kvh);
+  if (a.splits > 1 && a.offsets && q.q1 > q.q0 + q.rows) mark_rows(a, q.q0 + q.rows, q.q1, j.part, j.parts);
 }
 
 // keys first .. last - 1 (multiples of `step` but the last) of `most` that range `split` takes; used: ranges in all
@@ -653,7 +688,7 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_att_split(Args a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[kLds];
   __shared__ float s_m[NW][32], s_l[NW][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const Job job = job_of(a);
+  const Job job = job_of<kRowsW>(a, lane);
   const int s = job.s, kh = job.kh, split = job.split;
   if (s >= a.n) {
     rest_of_rows(a, job, Ge::EB);
@@ -838,12 +873,13 @@ __global__ __launch_bounds__(64 * kWavesR, 2) void paged_att_rows(Args a) {
   constexpr int NT = Ge::EB == 2 ? 2 : 1;  // score tiles a step (64 or 32 keys)
   constexpr int kStep = NT * kKeys;
   constexpr int kImg = kStep * Ge::RB;
+  constexpr int NS = 2;  // steps in the ring (three or four measured the same: the loads are not what it waits for)
   constexpr int kIt = kImg / 1024 / kWavesR;  // loads of one image a wave
   constexpr int kRowsL = kStep / kWavesR;     // image rows a wave loads
-  static_assert(kIt >= 1 && 4 * kImg <= 65536, "load_lds reaches 64 KB");
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * kImg];
+  static_assert(kIt >= 1 && NS >= 2 && NS * 2 * kImg <= 65536, "load_lds reaches 64 KB");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[NS * 2 * kImg];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Job job = job_of(a);
+  const Job job = job_of<kTileR>(a, lane);
   const int s = job.s, kh = job.kh, split = job.split;
   if (s >= a.n) {
     rest_of_rows(a, job, Ge::EB);
@@ -866,23 +902,24 @@ __global__ __launch_bounds__(64 * kWavesR, 2) void paged_att_rows(Args a) {
   const int t0 = rg.first / kStep, t1 = (rg.last + kStep - 1) / kStep;
   const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(lds));
   if (a.D != DP) {
-    clear_lds<T, DP>(lds, 4 * kImg, tid, 64 * kWavesR);
+    clear_lds<T, DP>(lds, NS * 2 * kImg, tid, 64 * kWavesR);
     __syncthreads();
   }
   const int safe = a.kn ? max(0, min(q.kv, q.st)) : q.kv;
   Pages pg;
-  uint32_t gaps = 0;  // bit of a buffer: a page of its keys is outside the pool
+  uint32_t gaps = 0;  // bit of a ring slot: a page of its keys is outside the pool
   pg.start(a, tab, (t0 * kStep) >> a.sh, lane);
   const auto issue = [&](int step) {
     const int j0 = step * kStep;
     pg.need(a, tab, j0 >> a.sh, (j0 + kStep - 1) >> a.sh, lane);
-    const uint32_t slot = (uint32_t)(step - t0) % 2u, d = at + slot * (2 * kImg);
+    const uint32_t slot = (uint32_t)(step - t0) % NS, d = at + slot * (2 * kImg);
     const bool gap = pg.any_bad(j0 >> a.sh, (min(q.kv, j0 + kStep) - 1) >> a.sh);
     gaps = (gaps & ~(1u << slot)) | ((uint32_t)gap << slot);
     load_tile<T, DP, kIt>(a, q, pg, kn, vn, kh, j0, wave * kRowsL, safe, d, d + kImg, lane);
   };
-  if (t0 < t1) issue(t0);
-  if (t0 + 1 < t1) issue(t0 + 1);
+#pragma unroll
+  for (int t = 0; t < NS - 1; ++t)
+    if (t0 + t < t1) issue(t0 + t);
   if (a.kn && split == 0) {
     const int i0 = (g0 + a.G - 1) / a.G, i1 = min(q.rows, (g0 + kTileR + a.G - 1) / a.G);
     write_chunk<T>(a, q, s, kn, vn, kh, i0, i1, tid, 64 * kWavesR);
@@ -892,33 +929,33 @@ __global__ __launch_bounds__(64 * kWavesR, 2) void paged_att_rows(Args a) {
   bool odd = false;  // a value that is not finite was scrubbed
   const int least = a.causal ? max(0, min(q.kv, q.st + g0 / a.G + 1)) : q.kv;  // keys the tile's first row sees
   for (int step = t0; step < t1; ++step) {
-    unsigned char* kt = lds + (uint32_t)(step - t0) % 2u * (2 * kImg);
+    const uint32_t slot = (uint32_t)(step - t0) % NS;
+    unsigned char* kt = lds + slot * (2 * kImg);
     unsigned char* vt = kt + kImg;
     const int j0 = step * kStep;
-    if (step + 1 < t1)
-      wait_loads<2 * kIt>();
+    if (step + NS - 1 <= t1)
+      wait_loads<(NS - 2) * 2 * kIt>();
     else
       wait_loads<0>();
     if (least < min(q.kv, j0 + kStep))
       odd |= scrub_image<T>(vt + wave * kRowsL * Ge::RB, kRowsL * Ge::RB, lane, 64);  // (what the wave has loaded)
-    wave_barrier();
-    if (!__all(j0 >= w.lim)) {
-      f32x16 sc[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) sc[t] = scores<T, DP>(w, kt + t * kKeys * Ge::RB, lane);
-      const bool gap = (gaps >> ((uint32_t)(step - t0) % 2u)) & 1u;
-      if (gap || !__all(j0 + kStep <= w.lim)) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-          mask_scores(sc[t], j0 + t * kKeys, w.lim, gap ? keys_there(a, tab, j0 + t * kKeys, q.kv, lane) : ~0u, lane);
-      }
-      soft_step<T, DP, NT>(w, sc, a.c);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) weigh<T, DP>(w, sc[t], vt + t * kKeys * Ge::RB, lane);
-    }
     wait_lds();
-    wave_barrier();  // (every wave has read the tile: the next loads may overwrite it)
-    if (step + 2 < t1) issue(step + 2);
+    // every wave's part of the step has landed, and every wave has read the step before: its slot is free
+    wave_barrier();
+    const bool gap = (gaps >> slot) & 1u;
+    if (step + NS - 1 < t1) issue(step + NS - 1);
+    if (__all(j0 >= w.lim)) continue;
+    f32x16 sc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) sc[t] = scores<T, DP>(w, kt + t * kKeys * Ge::RB, lane);
+    if (gap || !__all(j0 + kStep <= w.lim)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        mask_scores(sc[t], j0 + t * kKeys, w.lim, gap ? keys_there(a, tab, j0 + t * kKeys, q.kv, lane) : ~0u, lane);
+    }
+    soft_step<T, DP, NT>(w, sc, a.c);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) weigh<T, DP>(w, sc[t], vt + t * kKeys * Ge::RB, lane);
   }
   if (least < most && __syncthreads_or(odd))
     add_non_finite<T, DP>(w, a, q, kn, vn, tab, kh, max(t0, least / kStep) * kStep, min(most, t1 * kStep), lane);
@@ -933,7 +970,8 @@ __global__ __launch_bounds__(64 * kWavesR, 2) void paged_att_rows(Args a) {
 
 struct Plan {
   bool rows_kernel;
-  int tiles, splits, waves, range;
+  int64_t tiles, items;  // Args::tiles; work items but for splits and key heads
+  int splits, waves, range;
 };
 
 Plan plan_of(const mfl_paged_attention_args* p) {
@@ -942,15 +980,17 @@ Plan plan_of(const mfl_paged_attention_args* p) {
   const int64_t kv = p->max_kv < 1 ? 1 : p->max_kv;
   r.rows_kernel = M > 2 * kRowsW;
   const int64_t rows = r.rows_kernel ? kTileR : kRowsW, step = r.rows_kernel ? 2 * kKeys : kKeys;
-  r.tiles = (int)((M + rows - 1) / rows);
-  if (r.tiles < 1) r.tiles = 1;
-  r.waves = r.rows_kernel ? kWavesR : kv > 2 * kKeys && kv <= 512 ? 2 : 1;
-  // tiles that there are: packed sequences share p->total rows
-  int64_t base = p->n * r.tiles;
+  // tiles of a sequence; packed: of all together (they share p->total rows), and one behind the last
+  int64_t base;
   if (p->offsets) {
-    const int64_t few = (p->total * G + rows - 1) / rows + p->n;
-    if (few < base) base = few;
+    const int64_t most = p->n * ((M + rows - 1) / rows), few = (p->total * G + rows - 1) / rows + p->n;
+    base = few < most ? few : most;
+    r.items = r.tiles = base + 1;
+  } else {
+    r.tiles = (M + rows - 1) / rows;
+    base = r.items = p->n * r.tiles;
   }
+  r.waves = r.rows_kernel ? kWavesR : kv > 2 * kKeys && kv <= 512 ? 2 : 1;
   base *= p->kv_heads;
   if (base < 1) base = 1;
   // the split kernel reaches the memory's rate with some 8,192 ranges of one wave each, of at least 256 keys; up to
@@ -961,6 +1001,7 @@ Plan plan_of(const mfl_paged_attention_args* p) {
   range = (range + step - 1) / step * step;
   int64_t sp = (kv + range - 1) / range;
   if (sp > 512) sp = 512;
+  if (p->rows == 0) sp = 1;
   r.splits = (int)sp;
   r.range = (int)range;
   return r;
@@ -1001,15 +1042,14 @@ bool check(const mfl_paged_attention_args* p) {
   const int64_t M = p->rows * (p->heads / p->kv_heads);
   if (p->rows > (1ll << 30) || M > (1ll << 30) || p->n > (1ll << 30) || slots_of(p) * p->heads >= (1ll << 31)) return mfl_paged_error("%s: too many rows", who);
   const Plan pl = plan_of(p);
-  if ((p->n + 1) * pl.tiles * pl.splits * p->kv_heads >= (1ll << 31))
+  if (pl.items > (1ll << 30) || pl.items * pl.splits * p->kv_heads >= (1ll << 31))
     return mfl_paged_error("%s: too many sequences and rows for one launch", who);
   return true;
 }
 
 template <class T, int DP>
 int launch(const Args& a, const Plan& pl, hipStream_t st) {
-  const unsigned seqs = (unsigned)a.n + (a.offsets && (a.zero_tail || pl.splits > 1) ? 1u : 0u);
-  const dim3 grid(seqs * (unsigned)pl.tiles * (unsigned)pl.splits * (unsigned)a.kvh);
+  const dim3 grid((unsigned)pl.items * (unsigned)pl.splits * (unsigned)a.kvh);
   if (pl.rows_kernel)
     hipLaunchKernelGGL((paged_att_rows<T, DP>), grid, dim3(64 * kWavesR), 0, st, a);
   else if (pl.waves == 1)
@@ -1105,7 +1145,7 @@ int mfl_paged_attention(const mfl_paged_attention_args* p, void* stream) {
   a.width = (int)p->width;
   a.causal = p->causal != 0;
   a.splits = pl.splits;
-  a.tiles = pl.tiles;
+  a.tiles = (int)pl.tiles;
   a.zero_tail = p->offsets && p->zero_tail;
   a.total = p->total;
   a.slots = slots_of(p);
