@@ -368,7 +368,8 @@ bool check(const mfl_logits_args* p) {
   if (p->n < 0 || p->n > (1 << 24) || p->vocab < 0 || p->vocab > (1 << 30) || p->hist < 0 || p->hist > (1 << 30))
     return bad("%s: n %lld, vocab %lld, hist %lld", who, (long long)p->n, (long long)p->vocab, (long long)p->hist);
   if (!esize(p->dtype) || !esize(p->out_dtype)) return bad("%s: dtype tag (0 float32, 2 bfloat16, 3 float16)", who);
-  if (p->n * tiles_of(p) >= (1ll << 31)) return bad("%s: too many rows and tokens for one launch", who);
+  const Plan pl = plan_of(p);  // (a launch holds fewer than 2^32 threads)
+  if (p->n * pl.tiles * pl.threads >= (1ll << 32) || p->n * 64 >= (1ll << 32)) return bad("%s: too many rows and tokens for one launch", who);
   if (p->allowed_kind < 0 || p->allowed_kind > 2) return bad("%s: allowed_kind %lld", who, (long long)p->allowed_kind);
   if (p->allowed_kind && (p->allowed_rows < 1 || p->allowed_rows > (1 << 30)))
     return bad("%s: allowed_rows %lld", who, (long long)p->allowed_rows);

@@ -1042,7 +1042,8 @@ bool check(const mfl_paged_attention_args* p) {
   const int64_t M = p->rows * (p->heads / p->kv_heads);
   if (p->rows > (1ll << 30) || M > (1ll << 30) || p->n > (1ll << 30) || slots_of(p) * p->heads >= (1ll << 31)) return mfl_paged_error("%s: too many rows", who);
   const Plan pl = plan_of(p);
-  if (pl.items > (1ll << 30) || pl.items * pl.splits * p->kv_heads >= (1ll << 31))
+  // (a launch holds fewer than 2^32 threads)
+  if (pl.items > (1ll << 30) || pl.items * pl.splits * p->kv_heads * 64 * pl.waves >= (1ll << 32))
     return mfl_paged_error("%s: too many sequences and rows for one launch", who);
   return true;
 }

@@ -111,7 +111,8 @@ def test_damaged_entries_hold_nothing(dev):
 
 @pytest.mark.parametrize("n, width, pages, ps, seed", [(1, 1, 1, 1, 0), (5, 7, 40, 4, 1), (12, 40, 300, 1, 2),
                                                      (300, 9, 1500, 16, 3), (7, 300, 1025, 2, 4), (40, 20, 500, 32, 5),
-                                                     (1200, 3, 5000, 8, 6)])
+                                                     (1200, 3, 5000, 8, 6), (100, 100, 8192, 4, 7),
+                                                     (1024, 16, 8191, 16, 8), (3, 6000, 20000, 1, 9)])
 def test_random_histories(dev, n, width, pages, ps, seed):
     """Forks, cuts, growth and compactions in turn; now and then more is asked for than there is."""
     r = random.Random(seed)
