@@ -807,10 +807,11 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_att_split(Args a) {
 }
 
 // out = sum_i 2^(c (m_i - m)) O_i / sum_i 2^(c (m_i - m)) l_i over a row's ranges.  DP / 4 lanes hold a row's
-// columns; a workgroup takes 256 / (DP / 4) rows, or (WIDE: many ranges) one row whose ranges its groups share
+// columns; a workgroup of 256 takes 256 / (DP / 4) rows, one of 1,024 (WIDE: many ranges) one row whose ranges its
+// groups share
 template <class T, int DP, bool WIDE>
-__global__ __launch_bounds__(256) void paged_att_join(Args a) {
-  constexpr int kQ = DP / 4, kGr = 256 / kQ;
+__global__ __launch_bounds__(WIDE ? 1024 : 256) void paged_att_join(Args a) {
+  constexpr int kQ = DP / 4, kGr = (WIDE ? 1024 : 256) / kQ;
   __shared__ float s_m[kGr], s_l[kGr];
   __shared__ __attribute__((aligned(16))) float s_o[WIDE ? kGr : 1][DP];
   const int gr = threadIdx.x / kQ, col = threadIdx.x % kQ * 4;
@@ -1061,7 +1062,7 @@ int launch(const Args& a, const Plan& pl, hipStream_t st) {
     const long long rows = a.slots * a.heads;
     constexpr int kGr = 256 / (DP / 4);
     if (pl.splits > 16)
-      hipLaunchKernelGGL((paged_att_join<T, DP, true>), dim3((unsigned)rows), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((paged_att_join<T, DP, true>), dim3((unsigned)rows), dim3(1024), 0, st, a);
     else
       hipLaunchKernelGGL((paged_att_join<T, DP, false>), dim3((unsigned)((rows + kGr - 1) / kGr)), dim3(256), 0, st, a);
   }
