@@ -30,8 +30,8 @@ extern "C" {
  *
  * Rows: offsets NULL — `rows` rows of every sequence, sequence s's row i at s * *_seq + i * *_row (elements);
  * offsets (n + 1, int32, ascending) — sequence s has rows offsets[s] .. offsets[s + 1] of `total` packed rows
- * *_row apart, `rows` bounds their number (further ones are not computed), and rows behind offsets[n] are
- * set to zero when zero_tail, else left as they were.  q, k_new, v_new heads are *_head apart, the last
+ * *_row apart, `rows` bounds their number (further ones are neither computed nor written), and rows before
+ * offsets[0] or behind offsets[n] are set to zero when zero_tail, else left as they were.  q, k_new, v_new heads are *_head apart, the last
  * dimension contiguous, all strides multiples of 16 bytes; out is contiguous.
  * dtype: 0 float32, 2 bfloat16, 3 float16.  dim <= 128, a multiple of 16 bytes.  max_kv bounds kv_lens
  * for the choice of the launch only (a larger one is still computed in full).  workspace:

@@ -735,6 +735,7 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_att_split(Args a) {
     // the tile writes the tokens whose first row it holds
     const int i0 = (m0 + a.G - 1) / a.G, i1 = min(q.rows, (m0 + kRowsW + a.G - 1) / a.G);
     write_chunk<T>(a, q, s, kn, vn, kh, i0, i1, threadIdx.x, 64 * NW);
+    wait_loads<0>();  // (the loop's counts are of loads only)
   }
   Cols<T, DP> w;
   cols_init<T, DP>(w, a, q, qb, kh, m0, lane);
@@ -924,6 +925,7 @@ __global__ __launch_bounds__(64 * kWavesR, 2) void paged_att_rows(Args a) {
   if (a.kn && split == 0) {
     const int i0 = (g0 + a.G - 1) / a.G, i1 = min(q.rows, (g0 + kTileR + a.G - 1) / a.G);
     write_chunk<T>(a, q, s, kn, vn, kh, i0, i1, tid, 64 * kWavesR);
+    wait_loads<0>();  // (the loop's counts are of loads only)
   }
   Cols<T, DP> w;
   cols_init<T, DP>(w, a, q, qb, kh, m0, lane);
@@ -1112,8 +1114,9 @@ int mfl_paged_attention(const mfl_paged_attention_args* p, void* stream) {
   if (p->n == 0 || p->rows == 0) {
     if (!(p->offsets && p->zero_tail && p->total > 0)) return 0;
   }
-  // (without sequences only the rows behind them are set: an empty table has no address)
-  if (!p->out || (p->n > 0 && (!p->q || !p->k_pages || !p->v_pages || !p->table || !p->kv_lens))) {
+  // (what is empty has no address: a table without sequences or columns, a pool without pages)
+  if (!p->out || (p->n > 0 && (!p->q || !p->kv_lens || (p->width > 0 && !p->table) ||
+                               (p->pages > 0 && (!p->k_pages || !p->v_pages))))) {
     mfl_paged_error("mfl_paged_attention: NULL pointer");
     return 1;
   }

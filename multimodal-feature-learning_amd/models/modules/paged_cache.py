@@ -66,10 +66,10 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, *, k=None, v=None, star
     row i's are written to the pages at p, where p is in [0, kv_lens), and attended.  The positions written must
     lie in pages that no other sequence reads (``pages_update`` sees to it).
 
-    ``max_rows``: the largest number of rows of a packed sequence (rows beyond it are not computed; default:
-    total).  ``max_kv`` guides the launch only (default: what the table holds).  ``scale``: dim ** -0.5.
-    Returns ``out``, q's shape and type, contiguous; packed rows behind the last sequence are 0 in a new
-    tensor and stay as they were in a given one.  float32, bfloat16 and float16; dim up to 128, a multiple of
+    ``max_rows``: the largest number of rows of a packed sequence (rows beyond it are neither computed nor written;
+    default: total).  ``max_kv`` guides the launch only (default: what the table holds).  ``scale``: dim ** -0.5.
+    Returns ``out``, q's shape and type, contiguous; packed rows before the first sequence and behind the last are
+    0 in a new tensor and stay as they were in a given one.  float32, bfloat16 and float16; dim up to 128, a multiple of
     16 bytes; float32 statistics.  No gradients.
     """
     who = "paged_attention"
@@ -291,8 +291,7 @@ class PagedKVCache:
             raise ValueError(f"PagedKVCache: page_size {page_size} is no power of two")
         self.page_size, self.max_tokens = page_size, max_tokens
         width = max(1, (max_tokens + page_size - 1) // page_size)
-        # (every row's pages, and a copy of its last one while it still shares the original)
-        pages = rows * (width + 1) if pages is None else pages
+        pages = rows * width if pages is None else pages  # (no rows can hold more different ones)
         self.data = torch.zeros(layers, 2, pages, kv_heads, page_size, head_dim, dtype=dtype, device=device)
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(rows, dtype=torch.int32, device=device)

@@ -198,3 +198,29 @@ def test_dvc_inference_with_beams(dev):
     assert torch.equal(a[1], b[1])
     assert c[1].shape == a[1].shape and c[0]['pred_captions'].shape == a[0]['pred_captions'].shape
     assert bool(torch.isfinite(c[0]['pred_captions']).all())
+
+
+@pytest.mark.parametrize("kind", ["sparse", "multimodal"])
+def test_the_other_wrappers_with_beams(dev, golden, kind):
+    import test_dvc as T
+    g = golden("sparse_dvc_f64" if kind == "sparse" else "mm_dvc_f64")
+    model = T._load(T.build_sparse_dvc("cpu") if kind == "sparse" else T.build_mm_dvc("cpu"), g["state_dict"])
+    model = model.float().to(dev).eval()
+
+    def single(x):
+        if isinstance(x, torch.Tensor):
+            return x.to(dev).float() if x.is_floating_point() else x.to(dev)
+        if isinstance(x, dict):
+            return {k: single(v) for k, v in x.items()}
+        return [single(v) for v in x] if isinstance(x, list) else x
+
+    obj = single(dict(g["obj"]))
+    kw = dict(is_training=False, val_mode="one_by_one") if kind == "sparse" else dict(is_training=False)
+    with torch.no_grad():
+        a = model(obj, **kw)
+        model.caption_options = dict(beams=1)
+        b = model(obj, **kw)
+        model.caption_options = dict(beams=3, length_penalty=1.0)
+        c = model(obj, **kw)
+    assert torch.equal(a[1], b[1])
+    assert c[1].shape == a[1].shape and bool(torch.isfinite(c[0]['pred_captions']).all())

@@ -284,3 +284,46 @@ def test_empty_calls(dev):
     out = call({**z, "q": one, "offsets": off})
     assert bool((out == 0).all())
     assert bool((call({**d, "kv_lens": torch.zeros_like(d["kv_lens"])}) == 0).all())
+
+
+def test_no_table_and_no_pages(dev):
+    """A table without columns and a pool without pages: nothing is visible, nothing is written."""
+    d = up(make(2, 2, 4, 2, 64, 16, [5, 6], BF, 17, write=True), dev)
+    assert bool((call({**d, "table": d["table"][:, :0]}) == 0).all())
+    none = d["k_pages"][:0]
+    assert bool((call({**d, "k_pages": none, "v_pages": none}) == 0).all())
+
+
+@pytest.mark.parametrize("n", [65, 130])
+def test_packed_many_sequences(dev, n):
+    """More sequences than a wave has lanes, empty ones among them, rows before the first sequence."""
+    lens = [(i * 7) % 5 for i in range(n)]
+    packed = [2]
+    for x in lens:
+        packed.append(packed[-1] + x)
+    kv = [x + (i * 13) % 40 for i, x in enumerate(lens)]
+    for heads, kvh in ((4, 2), (32, 1)):
+        d = make(n, 0, heads, kvh, 64, 16, kv, BF, n, packed=packed, write=True)
+        g = up(d, dev)
+        out = call(g, max_rows=4)
+        check(out, d, g["k_pages"], g["v_pages"])
+        assert bool((out[:2] == 0).all()) and bool((out[packed[-1]:] == 0).all())
+
+
+def test_expanded_and_single_row_strides(dev):
+    """A query shared by all sequences (stride 0), and dimensions of one with arbitrary strides."""
+    d = make(3, 1, 4, 2, 64, 16, [9, 30, 17], BF, 18)
+    d["q"] = d["q"][:1].expand(3, -1, -1, -1)
+    check(call(up(d, dev)), d)
+    g = up(make(1, 1, 4, 2, 64, 16, [30], BF, 19), dev)
+    want = call(g)
+    odd = torch.as_strided(g["q"].contiguous(), (1, 1, 4, 64), (3, 5, 64, 1))
+    assert torch.equal(call({**g, "q": odd}), want)
+
+
+def test_sharers_of_one_page_read_the_same_keys(dev):
+    """Two sequences over the same pages, at different lengths."""
+    d = make(2, 1, 4, 4, 64, 16, [40, 40], FP, 20)
+    d["table"][1] = d["table"][0]
+    d["kv_lens"][1] = 35
+    check(call(up(d, dev)), d)
