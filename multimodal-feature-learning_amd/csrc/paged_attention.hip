@@ -148,13 +148,30 @@ __device__ __forceinline__ bool row_src(const Args& a, const Seq& q, const unsig
 
 // 16 bytes a lane from global memory to LDS at byte `dst` + 16 * lane (dst: wave-uniform, below 64 KB).
 // The loads count in vmcnt; nothing but wait_loads() waits for them
-__device__ __forceinline__ void load_lds(const unsigned char* base, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst)
-               : "memory", "m0");
-}
 __device__ __forceinline__ void load_lds(const unsigned char* src, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst)
                : "memory", "m0");
+}
+// N of them, load i from base + off[i] + 1024 i to dst + 1024 i (the offset in the instruction counts on both sides)
+template <int N>
+__device__ __forceinline__ void load_lds_run(const unsigned char* base, const uint32_t (&off)[N], uint32_t dst) {
+  static_assert(N == 1 || N == 2 || N == 4, "");
+  if constexpr (N == 4)
+    asm volatile(
+        "s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
+        "global_load_lds_dwordx4 %1, %4 offset:1024\n\tglobal_load_lds_dwordx4 %2, %4 offset:2048\n\t"
+        "global_load_lds_dwordx4 %3, %4 offset:3072" ::"v"(off[0]),
+        "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(dst)
+        : "memory", "m0");
+  else if constexpr (N == 2)
+    asm volatile(
+        "s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2\n\t"
+        "global_load_lds_dwordx4 %1, %2 offset:1024" ::"v"(off[0]),
+        "v"(off[1]), "s"(base), "s"(dst)
+        : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[0]), "s"(base), "s"(dst)
+                 : "memory", "m0");
 }
 // all but the last N vector memory operations of the wave are done
 template <int N>
@@ -196,36 +213,48 @@ struct Pages {
     }
   }
   __device__ __forceinline__ bool any_bad(int first, int last) const {
+    if (bad == 0ull) return false;
     const int w = last - first + 1;
     return ((bad >> (first - base)) & (w >= 64 ? ~0ull : (1ull << w) - 1ull)) != 0ull;
   }
 };
 
 // loads of 1 KB (64 lanes) for image rows r0 .. of keys j0 + r0 ..: IT of them for keys and values each, LDS images
-// at kd and vd.  `safe`: keys below it come from the pages and are there
+// at kd and vd.  `safe`: keys below it come from the pages and are there.  Where up to 16 rows lie in one page
+// (and a row has all DP columns) the run of their loads has one scalar address: what this loop issues
+// beside the loads is a third of a step's instructions otherwise
 template <class T, int DP, int IT>
 __device__ __forceinline__ void load_tile(const Args& a, const Seq& q, const Pages& pg, const unsigned char* kn,
                                           const unsigned char* vn, int kh, int j0, int r0, int safe, uint32_t kd,
                                           uint32_t vd, int lane) {
   typedef Geo<T, DP> Ge;
   constexpr int RP = 64 / Ge::NC;  // rows a load
-  const int rb = a.D * Ge::EB, nch = rb / 16;
+  constexpr int RN0 = RP >= 16 ? 1 : 16 / RP, RN1 = RN0 > 4 ? 4 : RN0, RN = RN1 > IT ? IT : RN1;  // loads a run
+  static_assert(IT % RN == 0, "");
   const int lr = lane / Ge::NC, cp = lane % Ge::NC;
   const int jb = j0 + r0;
-  const int e0 = jb >> a.sh, e1 = (jb + IT * RP - 1) >> a.sh;
-  if (jb + IT * RP <= safe && a.ps >= RP && !pg.any_bad(e0, e1)) {
+  const uint32_t d0 = r0 / RP * 1024;
+  if (jb + IT * RP <= safe && a.ps >= RN * RP && a.D == DP && !pg.any_bad(jb >> a.sh, (jb + IT * RP - 1) >> a.sh)) {
+    const uint32_t head = (uint32_t)a.ps * Ge::RB;  // bytes of one head's rows of a page
 #pragma unroll
-    for (int t = 0; t < IT; ++t) {
-      const int row = r0 + t * RP + lr;
-      const int j = jb + t * RP;
-      const int page = __builtin_amdgcn_readlane(pg.cur, (j >> a.sh) - pg.base);
-      const long long off = (((long long)page * a.kvh + kh) * a.ps + (j & (a.ps - 1))) * rb;
-      const int ck = cp ^ Ge::k_swz(row), cv = cp ^ Ge::v_swz(row);
-      if (ck < nch) load_lds(a.kp + off, (uint32_t)(lr * rb + ck * 16), kd + (r0 / RP + t) * 1024);
-      if (cv < nch) load_lds(a.vp + off, (uint32_t)(lr * rb + cv * 16), vd + (r0 / RP + t) * 1024);
+    for (int g = 0; g < IT / RN; ++g) {
+      const int j = jb + g * RN * RP;
+      const uint32_t page = __builtin_amdgcn_readlane(pg.cur, (j >> a.sh) - pg.base);
+      const unsigned long long off = (unsigned long long)(page * (uint32_t)a.kvh + (uint32_t)kh) * head +
+                                     (uint32_t)(j & (a.ps - 1)) * Ge::RB;
+      uint32_t ok[RN], ov[RN];
+#pragma unroll
+      for (int t = 0; t < RN; ++t) {
+        const int row = r0 + (g * RN + t) * RP + lr;
+        ok[t] = lr * Ge::RB + ((cp ^ Ge::k_swz(row)) << 4);
+        ov[t] = lr * Ge::RB + ((cp ^ Ge::v_swz(row)) << 4);
+      }
+      load_lds_run<RN>(a.kp + off, ok, kd + d0 + g * RN * 1024);
+      load_lds_run<RN>(a.vp + off, ov, vd + d0 + g * RN * 1024);
     }
   } else {
-#pragma unroll
+    const int rb = a.D * Ge::EB, nch = rb / 16;
+#pragma unroll 1
     for (int t = 0; t < IT; ++t) {
       const int row = r0 + t * RP + lr;
       const int j = j0 + row;
@@ -233,8 +262,8 @@ __device__ __forceinline__ void load_tile(const Args& a, const Seq& q, const Pag
       RowSrc r;
       row_src(a, q, kn, vn, kh, j, page, rb, r);
       const int ck = cp ^ Ge::k_swz(row), cv = cp ^ Ge::v_swz(row);
-      if (ck < nch) load_lds(r.k + ck * 16, kd + (r0 / RP + t) * 1024);
-      if (cv < nch) load_lds(r.v + cv * 16, vd + (r0 / RP + t) * 1024);
+      if (ck < nch) load_lds(r.k + ck * 16, kd + d0 + t * 1024);
+      if (cv < nch) load_lds(r.v + cv * 16, vd + d0 + t * 1024);
     }
   }
 }
@@ -1031,8 +1060,8 @@ bool check(const mfl_paged_attention_args* p) {
     return mfl_paged_error("%s: dim %lld (at most 128, a multiple of 16 bytes)", who, (long long)p->dim);
   if (p->page_size < 1 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)))
     return mfl_paged_error("%s: page_size %lld is no power of two up to 1024", who, (long long)p->page_size);
-  if (p->width * p->page_size > (1ll << 30) || p->pages > (1ll << 30))
-    return mfl_paged_error("%s: a table row of more than 2^30 tokens, or more than 2^30 pages", who);
+  if (p->width * p->page_size > (1ll << 30) || p->pages * p->kv_heads >= (1ll << 31))
+    return mfl_paged_error("%s: a table row of more than 2^30 tokens, or 2^31 pages times key heads", who);
   if (!(p->scale > 0.0) || !(p->scale < 1e30)) return mfl_paged_error("%s: scale must be positive and finite", who);
   if ((p->k_new == nullptr) != (p->v_new == nullptr))
     return mfl_paged_error("%s: k_new and v_new come together", who);
