@@ -173,12 +173,10 @@ __device__ __forceinline__ void finish(const Args& a, int row, const Stat& r) {
   if (a.logprob) a.logprob[row] = top == -INFINITY ? -INFINITY : top - lse;
 }
 
-constexpr uint32_t kNone = 0xffffffffu;  // no penalised value (a NaN that the penalties never make)
-
 template <class T, class O, int THREADS, int NCH>
 __global__ __launch_bounds__(THREADS, NCH == 1 ? 8 : 4) void logits_tile(Args a) {
   constexpr int kPass = THREADS * kV, kTile = kPass * NCH;
-  __shared__ __attribute__((aligned(16))) uint32_t value[kTile];  // penalised logits
+  __shared__ __attribute__((aligned(16))) float value[kTile];  // penalised logits, where count is not 0
   __shared__ __attribute__((aligned(16))) uint32_t count[kTile];
   const int row = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
   const int v0 = tile * kTile, nv = min(kTile, a.vocab - v0);
@@ -225,47 +223,38 @@ __global__ __launch_bounds__(THREADS, NCH == 1 ? 8 : 4) void logits_tile(Args a)
       for (int e = 0; e < kV; ++e) ok[c] |= ((w >> (8 * e)) & 0xffu ? 1u : 0u) << e;
     }
   }
-  bool any = false;
   if (len > 0) {
-    const uint4 none = {kNone, kNone, kNone, kNone}, zero = {0, 0, 0, 0};
+    const uint4 zero = {0, 0, 0, 0};
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int i = c * kPass + (int)threadIdx.x * kV;
       if (i >= nv) continue;
-      uint4* vp = reinterpret_cast<uint4*>(value + i);
       uint4* cp = reinterpret_cast<uint4*>(count + i);
-      vp[0] = none, vp[1] = none;
       cp[0] = zero, cp[1] = zero;
     }
     __syncthreads();
     const auto add = [&](int v) {
-      if ((unsigned)v < (unsigned)nv) {
-        atomicAdd(count + v, 1u);
-        any = true;
-      }
+      if ((unsigned)v < (unsigned)nv) atomicAdd(count + v, 1u);
     };
 #pragma unroll
     for (int t = 0; t < kTok; ++t) add(held[t] - v0);
     for (int j = kTok * THREADS + threadIdx.x; j < len; j += THREADS) add(tok[j] - v0);
-    any = __syncthreads_or(any);
-    if (any) {
-      const float rep = a.rep ? a.rep[row] : a.rep_s, pres = a.pres ? a.pres[row] : a.pres_s;
-      const float freq = a.freq ? a.freq[row] : a.freq_s;
-      const auto apply = [&](int v) {
-        if ((unsigned)v >= (unsigned)nv) return;
-        const uint32_t c = atomicOr(count + v, 0x80000000u);
-        if (c & 0x80000000u) return;  // (another occurrence has it)
-        const float l = (float)src[v];
-        float y = l > 0.f ? l / rep : l * rep;
-        y = y - pres;
-        y = y - freq * (float)c;
-        value[v] = __float_as_uint(y);
-      };
+    const float rep = a.rep ? a.rep[row] : a.rep_s, pres = a.pres ? a.pres[row] : a.pres_s;
+    const float freq = a.freq ? a.freq[row] : a.freq_s;
+    __syncthreads();
+    const auto apply = [&](int v) {
+      if ((unsigned)v >= (unsigned)nv) return;
+      const uint32_t c = atomicOr(count + v, 0x80000000u);
+      if (c & 0x80000000u) return;  // (another occurrence has it)
+      const float l = (float)src[v];
+      float y = l > 0.f ? l / rep : l * rep;
+      y = y - pres;
+      value[v] = y - freq * (float)c;
+    };
 #pragma unroll
-      for (int t = 0; t < kTok; ++t) apply(held[t] - v0);
-      for (int j = kTok * THREADS + threadIdx.x; j < len; j += THREADS) apply(tok[j] - v0);
-      __syncthreads();
-    }
+    for (int t = 0; t < kTok; ++t) apply(held[t] - v0);
+    for (int j = kTok * THREADS + threadIdx.x; j < len; j += THREADS) apply(tok[j] - v0);
+    __syncthreads();
   }
   const bool stats = a.best || a.lse || a.logprob;
   Stat t{0ull, -INFINITY, 0.f};
@@ -273,11 +262,13 @@ __global__ __launch_bounds__(THREADS, NCH == 1 ? 8 : 4) void logits_tile(Args a)
   for (int c = 0; c < NCH; ++c) {
     const int i = c * kPass + (int)threadIdx.x * kV, m = max(0, min(kV, nv - i));
     if (m > 0) {
-      if (any) {
+      if (len > 0) {
+        const uint4* cp = reinterpret_cast<const uint4*>(count + i);
+        const uint4 n0 = cp[0], n1 = cp[1];
+        const uint32_t n[kV] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+        if (n[0] | n[1] | n[2] | n[3] | n[4] | n[5] | n[6] | n[7]) {
 #pragma unroll
-        for (int e = 0; e < kV; ++e) {
-          const uint32_t y = value[i + e];
-          x[c][e] = y == kNone ? x[c][e] : __uint_as_float(y);
+          for (int e = 0; e < kV; ++e) x[c][e] = n[e] ? value[i + e] : x[c][e];
         }
       }
       if (a.bias) {
