@@ -14,14 +14,26 @@
 // The reference value m follows the maximum only when that has grown by more than 2^8 (any m gives the same
 // quotient): most steps then need no rescale of O and no exchange between lanes.
 //
-//   paged_att_split  few rows a (sequence, key head): a workgroup takes 32 rows and a range of the keys,
-//                    its two waves halves of it, each through its own ring of tiles in LDS; their (m, l, O) meet in LDS
+//   paged_att_split  few rows a (sequence, key head): a wave takes 32 rows and a range of the keys through its own
+//                    ring of tiles in LDS; for some hundred keys two waves take halves of one range and meet in LDS
 //   paged_att_rows   many rows: 4 waves of 32 rows share double-buffered tiles of 64 keys
 //   paged_att_join   key ranges of either: (m, l, O) of a row out of the workspace
 //
 // Keys and values go to LDS by global_load_lds (16 bytes a lane): no registers are held while the loads fly,
-// so a wave keeps 16 to 32 KB in flight.  Rows of one load lie in one page where the page holds as many
-// (4 rows at 256 bytes): its address is then scalar and the lane's offset constant.
+// so a wave keeps 16 to 32 KB in flight, and the rows of up to four loads that lie in one page have one
+// scalar address.
+//
+// Measured on one MI355X (a 1 GB copy moves 5.0 TB/s, an 8192^3 product runs at 1.19 PFLOP/s in bf16, 154 TFLOP/s
+// in fp32):
+//   24 single tokens over 1 .. 16,384 keys, 32 / 8 heads of 128, bf16: 181 us, 5.0 TB/s — the memory's rate
+//   one single token over 131,071 keys, 16 / 2 heads of 128, fp16: 34 us (3.9 TB/s; 8 us of it the join)
+//   2 x 4,096 rows over 6,001 / 12,288 keys, 32 / 8 heads of 128, bf16: 970 us, 0.98 PFLOP/s.  A wave's step of 64
+//   keys takes the matrix unit 1,024 cycles and the vector unit some 1,130 (32 exponentials a lane at a
+//   quarter of the rate); with two waves a SIMD they overlap in part.  Not the loads' bandwidth (the same tile
+//   loaded again and again takes as long; 96 % come from the L2), but issuing them was 9 % until runs shared an
+//   address.  Priorities for the matrix products, 8 waves a tile, rings of 3 and 4, steps of 32 and 128 keys, and
+//   a pipeline over steps (Q K of the next and P V of the last beside this one's exponentials) measured
+//   the same or slower: what they gain in overlap they lose in registers, and with them in waves.
 //
 // MFMA 32x32x16 (16-bit): A lane (h, r): row r = lane & 31, k 8h..8h+7 (h = lane >> 5); B the same with
 // columns; D register e: row 8 (e >> 2) + 4 h + (e & 3), column lane & 31.  The reduction of the second
@@ -837,11 +849,12 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_att_split(Args a) {
 }
 
 // out = sum_i 2^(c (m_i - m)) O_i / sum_i 2^(c (m_i - m)) l_i over a row's ranges.  DP / 4 lanes hold a row's
-// columns; a workgroup of 256 takes 256 / (DP / 4) rows, one of 1,024 (WIDE: many ranges) one row whose ranges its
-// groups share
-template <class T, int DP, bool WIDE>
-__global__ __launch_bounds__(WIDE ? 1024 : 256) void paged_att_join(Args a) {
-  constexpr int kQ = DP / 4, kGr = (WIDE ? 1024 : 256) / kQ;
+// columns; a workgroup takes 256 / (DP / 4) rows, or (WIDE threads, many ranges) one row whose ranges its groups
+// share: 1,024 threads while the rows alone do not fill the chip (512 ranges of 16 rows: 12 -> 8 us), else 256
+// (768 rows of up to 43 ranges: 12 -> 5 us)
+template <class T, int DP, int WIDE>
+__global__ __launch_bounds__(WIDE ? WIDE : 256) void paged_att_join(Args a) {
+  constexpr int kQ = DP / 4, kGr = (WIDE ? WIDE : 256) / kQ;
   __shared__ float s_m[kGr], s_l[kGr];
   __shared__ __attribute__((aligned(16))) float s_o[WIDE ? kGr : 1][DP];
   const int gr = threadIdx.x / kQ, col = threadIdx.x % kQ * 4;
@@ -1092,10 +1105,12 @@ int launch(const Args& a, const Plan& pl, hipStream_t st) {
   if (pl.splits > 1) {
     const long long rows = a.slots * a.heads;
     constexpr int kGr = 256 / (DP / 4);
-    if (pl.splits > 16)
-      hipLaunchKernelGGL((paged_att_join<T, DP, true>), dim3((unsigned)rows), dim3(1024), 0, st, a);
+    if (pl.splits > 16 && rows < 256)
+      hipLaunchKernelGGL((paged_att_join<T, DP, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, a);
+    else if (pl.splits > 16)
+      hipLaunchKernelGGL((paged_att_join<T, DP, 256>), dim3((unsigned)rows), dim3(256), 0, st, a);
     else
-      hipLaunchKernelGGL((paged_att_join<T, DP, false>), dim3((unsigned)((rows + kGr - 1) / kGr)), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((paged_att_join<T, DP, 0>), dim3((unsigned)((rows + kGr - 1) / kGr)), dim3(256), 0, st, a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
