@@ -327,3 +327,47 @@ def test_sharers_of_one_page_read_the_same_keys(dev):
     d["table"][1] = d["table"][0]
     d["kv_lens"][1] = 35
     check(call(up(d, dev)), d)
+
+
+@pytest.mark.parametrize("dtype, dim", [(BF, 64), (F32, 40), (FP, 128)], ids=["bf16", "fp32", "fp16"])
+@pytest.mark.parametrize("write", [False, True])
+def test_packed_rows_over_key_ranges(dev, dtype, dim, write):
+    """Packed chunks over caches of 0 to 3,000 keys: some sequences in several key ranges, some in one, rows beyond
+    max_rows, rows before the first sequence and behind the last, an empty sequence — for both kernels."""
+    packed = [3, 8, 8, 48, 49, 60]
+    kv = [3000, 40, 1500, 700, 11]
+    for heads, kvh in ((4, 2), (2, 2)):
+        d = make(5, 0, heads, kvh, dim, 32, kv, dtype, dim + heads, packed=packed, write=write)
+        g = up(d, dev)
+        mine = torch.full_like(g["q"], 3.0)
+        out = call({**g, "k_pages": g["k_pages"].clone(), "v_pages": g["v_pages"].clone()}, max_rows=35, max_kv=3000,
+                   out=mine)
+        lim = dict(max_rows=35)
+        ref, aux, _, _ = O.paged_attention(**d, **lim)
+        tol = tolerance(ref, aux, dtype, dim, 3000)
+        seen = torch.zeros(63, dtype=torch.bool)
+        for s in range(5):
+            seen[packed[s]:min(packed[s + 1], packed[s] + 35)] = True
+        err = (out.double().cpu() - ref).abs()
+        assert bool((err <= tol)[seen].all())
+        assert bool((out.cpu()[~seen] == 3).all())
+        full = call(g, max_kv=3000)
+        check(full, d, g["k_pages"], g["v_pages"])
+        assert bool((full[:3] == 0).all()) and bool((full[60:] == 0).all())
+
+
+def test_many_rows_of_many_ranges(dev):
+    """320 rows of up to 20 ranges each, joined by a workgroup a row; and 16 rows by a larger one."""
+    for n in (40, 2):
+        kv = [5000 - 120 * (i % 40) for i in range(n)]
+        kv[-1] = 30
+        d = make(n, 1, 8, 1, 32, 64, kv, BF, n)
+        check(call(up(d, dev), max_kv=5000), d)
+
+
+def test_chunk_over_key_ranges(dev):
+    """A chunk of 100 rows whose own keys lie in the last of several ranges."""
+    for dtype in (BF, F32):
+        d = make(2, 100, 2, 1, 64, 16, [2100, 900], dtype, 31, write=True)
+        g = up(d, dev)
+        check(call(g, max_kv=2100), d, g["k_pages"], g["v_pages"])
