@@ -12,6 +12,12 @@
 //   update_commit  the new table (a row finds its own free pages: block by the counts, then by rank), the new
 //                  reference counts, and the copies of the used tokens in every plane
 // and for the compaction: compact_count, compact_rank, compact_commit.
+//
+// Measured on one MI355X: a beam step of 112 rows (28 groups of 4, 300 pages, six layers, 1.6 MB copied) 9.8 us in
+// update_small, against 18 us in four launches; 256 rows of up to 16,000 tokens in a pool of 158,000 pages 18 us
+// in four (2.7 + 3.5 + 3.4 + 8.5), bound by their dependence on each other; the same with one workgroup per
+// pool would read its 640 KB of counts alone, twice.  The compaction of 8,192 pages of 128 KB, of which
+// 1,966 move: 10 us of ranks and 61 us of copies, 5.0 TB/s read and written — the rate of a large copy.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -24,6 +30,7 @@ constexpr int kT = 256;          // threads a workgroup
 constexpr int kBlock = 1024;     // pages whose free (live) count is one block sum
 constexpr int kCopyWgs = 2048;   // workgroups that share the copies (8 a CU)
 constexpr int kSmallT = 1024;    // update_small: threads, and rows at most
+// update_small's counts take 12 bytes of LDS a page, and each of its workgroups reads the whole table
 constexpr int kSmallPages = 8192, kSmallEntries = 16384, kSmallWgs = 256;
 
 struct Row {
