@@ -158,6 +158,10 @@ __device__ __forceinline__ bool row_src(const Args& a, const Seq& q, const unsig
   return true;
 }
 
+// (m0, which holds the LDS address, is a reserved register to the compiler and warned about in clobber lists; nothing
+// else in this file uses it)
+#pragma clang diagnostic ignored "-Winline-asm"
+
 // 16 bytes a lane from global memory to LDS at byte `dst` + 16 * lane (dst: wave-uniform, below 64 KB).
 // The loads count in vmcnt; nothing but wait_loads() waits for them
 __device__ __forceinline__ void load_lds(const unsigned char* src, uint32_t dst) {
@@ -281,7 +285,6 @@ __device__ __forceinline__ void load_tile(const Args& a, const Seq& q, const Pag
 }
 
 // chunks behind a row's D elements: zero once, the loads leave them alone
-template <class T, int DP>
 __device__ __forceinline__ void clear_lds(unsigned char* lds, int bytes, int tid, int threads) {
   for (int i = tid * 16; i < bytes; i += threads * 16) *reinterpret_cast<uint4*>(lds + i) = uint4{0, 0, 0, 0};
 }
@@ -754,7 +757,7 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_att_split(Args a) {
   unsigned char* ring = lds + wave * NS * kStage;
   const uint32_t ring_at = __builtin_amdgcn_readfirstlane(lds_at(ring));
   if (a.D != DP) {
-    clear_lds<T, DP>(ring, NS * kStage, lane, 64);
+    clear_lds(ring, NS * kStage, lane, 64);
     wait_lds();
   }
   const int safe = a.kn ? max(0, min(q.kv, q.st)) : q.kv;
@@ -946,7 +949,7 @@ __global__ __launch_bounds__(64 * kWavesR, 2) void paged_att_rows(Args a) {
   const int t0 = rg.first / kStep, t1 = (rg.last + kStep - 1) / kStep;
   const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(lds));
   if (a.D != DP) {
-    clear_lds<T, DP>(lds, NS * 2 * kImg, tid, 64 * kWavesR);
+    clear_lds(lds, NS * 2 * kImg, tid, 64 * kWavesR);
     __syncthreads();
   }
   const int safe = a.kn ? max(0, min(q.kv, q.st)) : q.kv;

@@ -11,7 +11,7 @@
 //   update_count   free pages counted a block; the rows' requests numbered
 //   update_commit  the new table (a row finds its own free pages: block by the counts, then by rank), the new
 //                  reference counts, and the copies of the used tokens in every plane
-// and for the compaction: compact_count, compact_rank, compact_commit.
+// and for the compaction compact_small, or compact_count, compact_rank and compact_commit.
 //
 // Measured on one MI355X: a beam step of 112 rows (28 groups of 4, 300 pages, six layers, 1.6 MB copied) 9.8 us in
 // update_small, against 18 us in four launches; 256 rows of up to 16,000 tokens in a pool of 158,000 pages 18 us
@@ -30,6 +30,9 @@ constexpr int kT = 256;          // threads a workgroup
 constexpr int kBlock = 1024;     // pages whose free (live) count is one block sum
 constexpr int kCopyWgs = 2048;   // workgroups that share the copies (8 a CU)
 constexpr int kSmallT = 1024;    // update_small: threads, and rows at most
+// compact_small saves two launches (4,000 pages of 24 KB: 20 -> 15 us), but its copies begin late and reach less of
+// the memory's rate (8,192 pages of 128 KB: 71 -> 78 us)
+constexpr int64_t kSmallBytes = 256ll << 20;
 // update_small's counts take 12 bytes of LDS a page, and each of its workgroups reads the whole table
 constexpr int kSmallPages = 8192, kSmallEntries = 16384, kSmallWgs = 256;
 
@@ -434,10 +437,57 @@ __global__ __launch_bounds__(kT) void compact_rank(Cmp a) {
   }
 }
 
-__device__ __forceinline__ void copy_page(unsigned char* base, long long page_bytes, int src, int dst) {
+__device__ __forceinline__ void copy_page(unsigned char* base, long long page_bytes, int src, int dst, int tid,
+                                          int threads) {
   const unsigned char* f = base + src * page_bytes;
   unsigned char* t = base + dst * page_bytes;
-  for (long long i = threadIdx.x * 16; i < page_bytes; i += kT * 16) copy16(t + i, f + i);
+  for (long long i = tid * 16; i < page_bytes; i += threads * 16) copy16(t + i, f + i);
+}
+
+// pages <= kSmallPages: every workgroup ranks all pages in its LDS, writes its share of the outputs and does its
+// share of the copies
+__global__ __launch_bounds__(kSmallT) void compact_small(Cmp a) {
+  extern __shared__ short lds16[];  // (16 bits: two workgroups a CU, which the copies need)
+  short *to = lds16, *src = to + a.pages, *dst = src + a.pages;  // to[x]: where page x goes (-1: free)
+  const int tid = threadIdx.x, wg = blockIdx.x, wgs = gridDim.x;
+  const int run = (a.pages + kSmallT - 1) / kSmallT, x0 = min(a.pages, tid * run), x1 = min(a.pages, x0 + run);
+  uint32_t on = 0;  // bit i: page x0 + i lives (run <= 8)
+  for (int x = x0; x < x1; ++x) on |= (uint32_t)(a.refs[x] > 0) << (x - x0);
+  int live;
+  int before = block_scan<kSmallT>((int)__popc(on), live);
+  int v = 0;
+  for (int x = x0; x < x1; ++x) v += ((on >> (x - x0)) & 1u) && x < live;
+  const int below = block_sum<kSmallT>(v), moved = live - below;
+  for (int x = x0; x < x1; ++x) {
+    const bool o = (on >> (x - x0)) & 1u;
+    if (o && x >= live) src[before - below] = (short)x;
+    if (!o && x < live) dst[x - before] = (short)x;
+    to[x] = (short)(o ? (x < live ? x : -2 - (before - below)) : -1);
+    before += o;
+  }
+  __syncthreads();
+  if (wg == 0 && tid == 0) a.live_out[0] = live;
+  for (int x = wg * kSmallT + tid; x < a.pages; x += wgs * kSmallT) {
+    const int t = to[x];
+    a.remap_out[x] = t < -1 ? dst[-2 - t] : t;
+    if (x >= live)
+      a.refs_out[x] = 0;
+    else if (t >= 0)
+      a.refs_out[x] = a.refs[x];
+  }
+  for (int k = wg * kSmallT + tid; k < moved; k += wgs * kSmallT) a.refs_out[dst[k]] = a.refs[src[k]];
+  for (long long e = (long long)wg * kSmallT + tid; e < a.entries; e += (long long)wgs * kSmallT) {
+    const int x = a.table[e];
+    const int t = (unsigned)x < (unsigned)a.pages ? to[x] : -1;
+    a.table_out[e] = t < -1 ? dst[-2 - t] : t;
+  }
+  if (!a.data) return;
+  const long long plane = a.page_bytes * a.pages;
+  const int part = tid >> 8, lane = tid & 255;  // a quarter of the workgroup takes a page of one plane
+  for (long long e = (long long)wg * 4 + part; e < (long long)moved * a.planes; e += (long long)wgs * 4) {
+    const int k = (int)(e / a.planes), pl = (int)(e % a.planes);
+    copy_page(a.data + pl * plane, a.page_bytes, src[k], dst[k], lane, 256);
+  }
 }
 
 __global__ __launch_bounds__(kT) void compact_commit(Cmp a) {
@@ -460,7 +510,7 @@ __global__ __launch_bounds__(kT) void compact_commit(Cmp a) {
   const long long plane = a.page_bytes * a.pages;
   for (long long e = blockIdx.x; e < (long long)moved * a.planes; e += gridDim.x) {
     const int k = (int)(e / a.planes), pl = (int)(e % a.planes);
-    copy_page(a.data + pl * plane, a.page_bytes, a.src[k], a.dst[k]);
+    copy_page(a.data + pl * plane, a.page_bytes, a.src[k], a.dst[k], threadIdx.x, kT);
   }
 }
 
@@ -470,7 +520,7 @@ __global__ __launch_bounds__(kT) void pages_copy(const int* src, const int* dst,
   for (long long e = blockIdx.x; e < count * planes; e += gridDim.x) {
     const int f = src[e / planes], t = dst[e / planes];
     if ((unsigned)f >= (unsigned)pages || (unsigned)t >= (unsigned)pages) continue;
-    copy_page(data + (e % planes) * plane, page_bytes, f, t);
+    copy_page(data + (e % planes) * plane, page_bytes, f, t, threadIdx.x, kT);
   }
 }
 
@@ -591,6 +641,11 @@ int mfl_pages_compact(const int32_t* table, int64_t entries, const int32_t* refs
   a.counts = reinterpret_cast<int*>(ws), ws += pad16(a.blocks);
   a.moved = reinterpret_cast<int*>(ws);
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (pages <= kSmallPages && (!data || pages * planes * page_bytes <= kSmallBytes)) {
+    const unsigned wgs = data ? 2 * kSmallWgs : 8;  // (how many pages move is known on the device alone)
+    hipLaunchKernelGGL(compact_small, dim3(wgs), dim3(kSmallT), (size_t)(pages > 0 ? pages : 1) * 6, st, a);
+    return launched(who) ? 0 : 1;
+  }
   if (a.blocks > 0) hipLaunchKernelGGL(compact_count, dim3((unsigned)a.blocks), dim3(kT), 0, st, a);
   hipLaunchKernelGGL(compact_rank, dim3((unsigned)(a.blocks > 0 ? a.blocks : 1)), dim3(kT), 0, st, a);
   hipLaunchKernelGGL(compact_commit, dim3(kCopyWgs), dim3(kT), 0, st, a);

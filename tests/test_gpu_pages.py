@@ -253,3 +253,17 @@ def test_cache_runs_a_beam_search_of_chunks(dev):
     step([1] * n, [r.randrange(n) for _ in range(n)])
     cache.update(new_lens=i32([0] * n, dev))
     assert int(cache.refs.abs().sum()) == 0
+
+
+def test_compaction_of_a_large_pool(dev):
+    """More than 256 MB of pages (the ranks in launches of their own), few pages enough for one workgroup's."""
+    r = random.Random(1)
+    pages = 600
+    data = torch.randint(-9, 9, (2, 2, pages, 4, 64, 256), dtype=torch.int16, device=dev).view(torch.bfloat16)
+    refs = [int(r.random() < 0.5) for _ in range(pages)]
+    table = [x for x in range(pages) if refs[x]]
+    want = data.clone()
+    t, f, remap, live = pc.pages_compact(data, i32(table, dev), i32(refs, dev))
+    ot, of, orm, ol = O.pages_compact([table], refs, want)
+    assert t.tolist() == ot[0] and f.tolist() == of and remap.tolist() == orm and int(live) == ol
+    assert torch.equal(data.view(torch.int16), want.view(torch.int16))
