@@ -33,8 +33,12 @@ namespace {
 
 constexpr int kV = 8;                 // tokens a thread
 constexpr int kFew = 256, kMany = 1024;  // threads a workgroup: short / long histories
-constexpr int kLongHistory = 512;
-constexpr int kFewRows = 512;         // rows of which one-tile workgroups are no more than two a CU
+// (tokens of history: 256 x 128,005 takes 65 us in small tiles and 68 in large ones at 800, 91 and 74 at 4,096;
+// 32 x 50,000 takes 10.1 and 10.4, 15.4 and 10.9)
+constexpr int kLongHistory = 2048;
+// rows of up to 16,384 tokens that are one tile each: while all of their workgroups run at once, two a CU of one
+// pass (512 x 3,000: 7.8 us, 9.2 in tiles and a join), one of two (256 x 10,000: 8.2, 10; 300 x 10,000: 14.1, 10.6)
+constexpr int kFewRows = 512, kFewRows2 = 256;
 constexpr int kTok = 4;               // tokens of the history a thread holds
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -347,9 +351,10 @@ struct Plan {
 
 Plan plan_of(const mfl_logits_args* p) {
   Plan r{p->hist > kLongHistory ? kMany : kFew, 1, 0};
-  if (p->n <= kFewRows && p->vocab <= 2 * kMany * kV) {
+  const int passes = p->vocab <= kMany * kV ? 1 : 2;
+  if (p->n <= (passes == 1 ? kFewRows : kFewRows2) && p->vocab <= 2 * kMany * kV) {
     r.threads = p->vocab <= kFew * kV ? kFew : kMany;
-    r.passes = p->vocab <= kMany * kV ? 1 : 2;
+    r.passes = passes;
   }
   const int64_t tile = (int64_t)r.threads * r.passes * kV;
   r.tiles = (int)((p->vocab + tile - 1) / tile);

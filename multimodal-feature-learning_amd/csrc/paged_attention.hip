@@ -719,8 +719,9 @@ __device__ __forceinline__ Range range_of(const Args& a, int most, int split, in
   return r;
 }
 
+// (two waves a SIMD: left to itself the compiler keeps O in accumulation registers, and one wave fits at DP = 128)
 template <class T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void paged_att_split(Args a) {
+__global__ __launch_bounds__(64 * NW, NW == 1 ? 2 : 1) void paged_att_split(Args a) {
   typedef Geo<T, DP> Ge;
   constexpr int kImg = kKeys * Ge::RB;  // one 32-row image
   constexpr int kStage = 2 * kImg;      // keys and values
@@ -896,6 +897,7 @@ __global__ __launch_bounds__(WIDE ? WIDE : 256) void paged_att_join(Args a) {
     const float base = mx == -INFINITY ? 0.f : mx * a.c;
     l = 0.f;
     o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int i = 0; i < kGr; ++i) {
       const float f = __builtin_amdgcn_exp2f(fmaf(s_m[i], a.c, -base));
       l += s_l[i] * f;
@@ -1016,17 +1018,31 @@ __global__ __launch_bounds__(64 * kWavesR, 2) void paged_att_rows(Args a) {
   }
 }
 
+int dp_of(int64_t dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+
 struct Plan {
   bool rows_kernel;
   int64_t tiles, items;  // Args::tiles; work items but for splits and key heads
   int splits, waves, range;
 };
 
+// Which kernel, and into how many ranges the keys are cut.  Measured on one MI355X, us without -> with the rule:
+//   more than 32 rows a (sequence, key head): paged_att_rows; 33 .. 64 as two tiles of paged_att_split read the keys
+//     twice (128 x 8 heads x 36 rows over 4,096 keys 489 -> 379; 28 x 12 x 33 over 60: 12.2 -> 9.6)
+//   paged_att_split: the ranges that fill one wave a SIMD (1,024), of at least 64 keys (8 waves over 768 keys:
+//     16.2 -> 9.9, over 8,192: 18.4 -> 14.2; 64 over 2,048: 17.5 -> 13.4), all of them in one round (192 over 2,048 in
+//     960 waves 37, in 1,152 49).  Where that leaves a range of more than 1,024 keys, more and shorter ones
+//     (of 512 keys, or 8,192 in all) even out sequences of different lengths: 24 of up to 16,384 keys in ranges of 2,731
+//     would wait for the longest.  Two ranges of one row tile are two waves of one workgroup, which needs no join
+//     (384 over 512 keys: 25 -> 22), but never more than two (192 over 512 keys: 17.4 in two waves, 15.2 in ranges)
+//   paged_att_rows: a workgroup a CU for ranges of 128 keys and more, all that the chip holds for 384 and more (8
+//     over 1,024 keys: 20.8 -> 13.2; 32 over 16,384: 71 -> 55), but some 1,024 where ranges would be longer than 1,024
+//     keys, for unequal lengths again (packed chunks of up to 64 over 8,192: 68 -> 53)
 Plan plan_of(const mfl_paged_attention_args* p) {
   Plan r{};
   const int64_t G = p->heads / p->kv_heads, M = p->rows * G;
   const int64_t kv = p->max_kv < 1 ? 1 : p->max_kv;
-  r.rows_kernel = M > 2 * kRowsW;
+  r.rows_kernel = M > kRowsW;
   const int64_t rows = r.rows_kernel ? kTileR : kRowsW, step = r.rows_kernel ? 2 * kKeys : kKeys;
   // tiles of a sequence; packed: of all together (they share p->total rows), and one behind the last
   int64_t base;
@@ -1038,24 +1054,38 @@ Plan plan_of(const mfl_paged_attention_args* p) {
     r.tiles = (M + rows - 1) / rows;
     base = r.items = p->n * r.tiles;
   }
-  r.waves = r.rows_kernel ? kWavesR : kv > 2 * kKeys && kv <= 512 ? 2 : 1;
   base *= p->kv_heads;
   if (base < 1) base = 1;
-  // the split kernel reaches the memory's rate with some 8,192 ranges of one wave each, of at least 256 keys; up to
-  // 512 keys two waves share a range instead, which needs no join
-  const int64_t least = r.rows_kernel ? 512 : kv <= 512 ? 512 : 256, want = r.rows_kernel ? 1024 : 8192;
-  int64_t range = kv / ((want + base - 1) / base);
-  if (range < least) range = least;
-  range = (range + step - 1) / step * step;
-  int64_t sp = (kv + range - 1) / range;
+  const int64_t all = (1023 + base) / base;  // ranges of a tile that make 1,024 in all
+  int64_t sp;
+  if (!r.rows_kernel) {
+    const int64_t fill = base < 1024 ? 1024 / base : 1;
+    int64_t range = (kv + fill - 1) / fill;
+    if (range > 1024) range = kv * base / 8192 < 512 ? 512 : kv * base / 8192;
+    if (range < 2 * kKeys) range = 2 * kKeys;
+    sp = (kv + range - 1) / range;
+    r.waves = sp == 2 && fill > 1 ? 2 : 1;
+    if (r.waves == 2) sp = 1;
+  } else {
+    r.waves = kWavesR;
+    const int64_t slots = dp_of(p->dim) == 128 ? 512 : 768;  // workgroups the chip holds at once
+    if (4 * base <= slots) {
+      const int64_t cus = kv / 128 < 192 / base ? kv / 128 : 192 / base;
+      const int64_t held = kv / 384 < slots / base ? kv / 384 : slots / base;
+      sp = cus > held ? cus : held;
+      if (sp < 1) sp = 1;
+      if (kv / sp > 1024 && sp < all) sp = all;
+    } else {
+      const int64_t least = 2 * base < slots ? 512 : 1024;
+      sp = kv / least < all ? kv / least : all;
+    }
+  }
+  if (sp < 1 || p->rows == 0) sp = 1;
   if (sp > 512) sp = 512;
-  if (p->rows == 0) sp = 1;
   r.splits = (int)sp;
-  r.range = (int)range;
+  r.range = (int)(((kv + sp - 1) / sp + step - 1) / step * step);
   return r;
 }
-
-int dp_of(int64_t dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 
 int64_t slots_of(const mfl_paged_attention_args* p) { return p->offsets ? p->total : p->n * p->rows; }
 

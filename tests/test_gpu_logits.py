@@ -111,6 +111,12 @@ def test_penalties(dev, n, vocab, hist, dtype):
     check({**make(n, vocab, hist, n + vocab + 1, dtype, bias="rows"), **PEN}, dev, out_dtype=dtype)
 
 
+@pytest.mark.parametrize("n, vocab, hist", [(2, 20001, 2048), (2, 20001, 2049), (513, 2500, 5), (257, 9000, 20)])
+def test_ways_to_cut_a_row(dev, n, vocab, hist):
+    """Small and large tiles for histories of each side, rows in one tile and in several."""
+    check({**make(n, vocab, hist, n + hist), **PEN}, dev)
+
+
 @pytest.mark.parametrize("allowed", ["one", "rows", "states", "one-bits", "rows-bits", "states-bits"])
 @pytest.mark.parametrize("vocab", [31, 1000, 8200, 20001])
 def test_masks(dev, vocab, allowed):

@@ -371,3 +371,15 @@ def test_chunk_over_key_ranges(dev):
         d = make(2, 100, 2, 1, 64, 16, [2100, 900], dtype, 31, write=True)
         g = up(d, dev)
         check(call(g, max_kv=2100), d, g["k_pages"], g["v_pages"])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("n, heads, kvh, dim, rows, kv", [
+    (64, 8, 8, 32, 1, [1 + 699 * i // 63 for i in range(64)]),  # two waves of some hundred keys each
+    (3, 64, 64, 16, 1, [6000, 1, 513]),                         # more ranges than run at once
+    (1, 2, 2, 128, 2, [400]),                                   # ranges of 64 keys
+    (1, 8, 1, 64, 5, [1500]),                                   # 40 rows of one key head: a tile of 128
+], ids=["two-waves", "rounds", "short", "rows"])
+def test_ways_to_cut_the_keys(dev, n, heads, kvh, dim, rows, kv, dtype):
+    d = make(n, rows, heads, kvh, dim, 16, kv, dtype, seed=heads + dim)
+    check(call(up(d, dev), max_kv=max(kv)), d)
