@@ -15,8 +15,8 @@
 // quotient): most steps then need no rescale of O and no exchange between lanes.
 //
 //   paged_att_split  few rows a (sequence, key head): a wave takes 32 rows and a range of the keys through its own
-//                    ring of tiles in LDS; for some hundred keys two waves take halves of one range and meet in LDS
-//   paged_att_rows   many rows: 4 waves of 32 rows share double-buffered tiles of 64 keys
+//                    ring of tiles in LDS; where the keys make two ranges, two waves of a workgroup take one each and meet in LDS
+//   paged_att_rows   more rows: 4 waves of 32 rows share double-buffered tiles of 64 keys
 //   paged_att_join   key ranges of either: (m, l, O) of a row out of the workspace
 //
 // Keys and values go to LDS by global_load_lds (16 bytes a lane): no registers are held while the loads fly,
@@ -25,8 +25,8 @@
 //
 // Measured on one MI355X (a 1 GB copy moves 5.0 TB/s, an 8192^3 product runs at 1.19 PFLOP/s in bf16, 154 TFLOP/s
 // in fp32):
-//   24 single tokens over 1 .. 16,384 keys, 32 / 8 heads of 128, bf16: 181 us, 5.0 TB/s — the memory's rate
-//   one single token over 131,071 keys, 16 / 2 heads of 128, fp16: 34 us (3.9 TB/s; 8 us of it the join)
+//   24 single tokens over 1 .. 16,384 keys, 32 / 8 heads of 128, bf16: 178 us, 5.1 TB/s — the memory's rate
+//   one single token over 131,071 keys, 16 / 2 heads of 128, fp16: 31 us (4.3 TB/s; 5 us of it the join)
 //   2 x 4,096 rows over 6,001 / 12,288 keys, 32 / 8 heads of 128, bf16: 970 us, 0.98 PFLOP/s.  A wave's step of 64
 //   keys takes the matrix unit 1,024 cycles and the vector unit some 1,130 (32 exponentials a lane at a
 //   quarter of the rate); with two waves a SIMD they overlap in part.  Not the loads' bandwidth (the same tile
@@ -853,22 +853,35 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 2 : 1) void paged_att_split(Args
 }
 
 // out = sum_i 2^(c (m_i - m)) O_i / sum_i 2^(c (m_i - m)) l_i over a row's ranges.  DP / 4 lanes hold a row's
-// columns; a workgroup takes 256 / (DP / 4) rows, or (WIDE threads, many ranges) one row whose ranges its groups
-// share: 1,024 threads while the rows alone do not fill the chip (512 ranges of 16 rows: 12 -> 8 us), else 256
-// (768 rows of up to 43 ranges: 12 -> 5 us)
-template <class T, int DP, int WIDE>
-__global__ __launch_bounds__(WIDE ? WIDE : 256) void paged_att_join(Args a) {
-  constexpr int kQ = DP / 4, kGr = (WIDE ? WIDE : 256) / kQ;
-  __shared__ float s_m[kGr], s_l[kGr];
-  __shared__ __attribute__((aligned(16))) float s_o[WIDE ? kGr : 1][DP];
-  const int gr = threadIdx.x / kQ, col = threadIdx.x % kQ * 4;
+// columns; a workgroup takes 256 / (DP / 4) rows, or (WIDE: more than 16 ranges) 32 columns of one row, whose ranges its
+// 32 groups of 8 lanes share (16 rows of 512 ranges: 59 -> 5 us, 768 rows of up to 43: 12 -> 6.  Fewer ranges leave its
+// groups idle: 32 rows of 12 ranges would gain 0.5 us, 4,096 of 16 lose 8)
+struct JoinSum {
+  float m, l;
+  f32x4 o;
+};
+__device__ __forceinline__ void join_add(JoinSum& w, float m, float l, const f32x4& o, float c) {
+  const float mn = fmaxf(w.m, m), base = mn == -INFINITY ? 0.f : mn * c;
+  const float f0 = __builtin_amdgcn_exp2f(fmaf(w.m, c, -base)), f1 = __builtin_amdgcn_exp2f(fmaf(m, c, -base));
+  w.m = mn;
+  w.l = w.l * f0 + l * f1;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w.o[k] = w.o[k] * f0 + o[k] * f1;
+}
+
+template <class T, int DP, bool WIDE>
+__global__ __launch_bounds__(256) void paged_att_join(Args a) {
+  constexpr int kQ = WIDE ? 8 : DP / 4, kGr = 256 / kQ, kParts = WIDE ? DP / 32 : 1, kWv = 4;
+  __shared__ float s_m[kWv], s_l[kWv];
+  __shared__ __attribute__((aligned(16))) f32x4 s_o[kWv][kQ];
+  const int gr = threadIdx.x / kQ, x = threadIdx.x % kQ;
+  const int col = (WIDE ? (int)(blockIdx.x % kParts) * 32 : 0) + x * 4;
   const long long sh = a.slots * a.heads;
-  const long long id = WIDE ? (long long)blockIdx.x : (long long)blockIdx.x * kGr + gr;
+  const long long id = WIDE ? (long long)(blockIdx.x / kParts) : (long long)blockIdx.x * kGr + gr;
   const Part p = part_of(a, 0, DP);
   const int used = id < sh ? min(p.used[id], a.splits) : 0;  // (offsets that do not ascend leave rows unmarked)
   if (WIDE && used <= 1) return;
-  float m = -INFINITY, l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  JoinSum w = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
   if (used > 1) {
     const int i0 = WIDE ? gr : 0;
     constexpr int kStep = WIDE ? kGr : 1;
@@ -876,40 +889,36 @@ __global__ __launch_bounds__(WIDE ? WIDE : 256) void paged_att_join(Args a) {
     for (int i = i0; i < used; i += kStep) {
       const float mi = p.ml[(i * sh + id) * 2], li = p.ml[(i * sh + id) * 2 + 1];
       const f32x4 v = *reinterpret_cast<const f32x4*>(p.o + (i * sh + id) * DP + col);  // (behind D: not used)
-      const float mn = fmaxf(m, mi), base = mn == -INFINITY ? 0.f : mn * a.c;
-      const float f0 = __builtin_amdgcn_exp2f(fmaf(m, a.c, -base)), f1 = __builtin_amdgcn_exp2f(fmaf(mi, a.c, -base));
-      m = mn;
-      l = l * f0 + li * f1;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] = o[k] * f0 + v[k] * f1;
+      join_add(w, mi, li, v, a.c);
     }
   }
   if constexpr (WIDE) {
-    if (col == 0) {
-      s_m[gr] = m;
-      s_l[gr] = l;
+#pragma unroll
+    for (int d = kQ; d < 64; d <<= 1) {
+      const float m = __shfl_xor(w.m, d), l = __shfl_xor(w.l, d);
+      f32x4 o;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = __shfl_xor(w.o[k], d);
+      join_add(w, m, l, o, a.c);
     }
-    *reinterpret_cast<f32x4*>(&s_o[gr][col]) = o;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) < kQ) {
+      if (x == 0) {
+        s_m[wave] = w.m;
+        s_l[wave] = w.l;
+      }
+      s_o[wave][x] = w.o;
+    }
     __syncthreads();
     if (gr != 0) return;
-    float mx = -INFINITY;
-    for (int i = 0; i < kGr; ++i) mx = fmaxf(mx, s_m[i]);
-    const float base = mx == -INFINITY ? 0.f : mx * a.c;
-    l = 0.f;
-    o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int i = 0; i < kGr; ++i) {
-      const float f = __builtin_amdgcn_exp2f(fmaf(s_m[i], a.c, -base));
-      l += s_l[i] * f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] += s_o[i][col + k] * f;
-    }
+    for (int i = 1; i < kWv; ++i) join_add(w, s_m[i], s_l[i], s_o[i][x], a.c);
   }
   if (used <= 1 || col >= a.D) return;
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const float inv = w.l > 0.f ? 1.f / w.l : (w.l == 0.f ? 0.f : w.l);
   float v[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = o[k] * inv;
+  for (int k = 0; k < 4; ++k) v[k] = w.o[k] * inv;
   store4<T>(a.out + (id * (long long)a.D + col) * (long long)sizeof(T), v);
 }
 
@@ -1121,7 +1130,8 @@ bool check(const mfl_paged_attention_args* p) {
   if (p->rows > (1ll << 30) || M > (1ll << 30) || p->n > (1ll << 30) || slots_of(p) * p->heads >= (1ll << 31)) return mfl_paged_error("%s: too many rows", who);
   const Plan pl = plan_of(p);
   // (a launch holds fewer than 2^32 threads)
-  if (pl.items > (1ll << 30) || pl.items * pl.splits * p->kv_heads * 64 * pl.waves >= (1ll << 32))
+  if (pl.items > (1ll << 30) || pl.items * pl.splits * p->kv_heads * 64 * pl.waves >= (1ll << 32) ||
+      (pl.splits > 1 && (slots_of(p) * p->heads + 256) * (dp_of(p->dim) / 4) >= (1ll << 32)))
     return mfl_paged_error("%s: too many sequences and rows for one launch", who);
   return true;
 }
@@ -1138,12 +1148,10 @@ int launch(const Args& a, const Plan& pl, hipStream_t st) {
   if (pl.splits > 1) {
     const long long rows = a.slots * a.heads;
     constexpr int kGr = 256 / (DP / 4);
-    if (pl.splits > 16 && rows < 256)
-      hipLaunchKernelGGL((paged_att_join<T, DP, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, a);
-    else if (pl.splits > 16)
-      hipLaunchKernelGGL((paged_att_join<T, DP, 256>), dim3((unsigned)rows), dim3(256), 0, st, a);
+    if (pl.splits > 16 && rows < (1 << 22))  // (a launch holds fewer than 2^32 threads)
+      hipLaunchKernelGGL((paged_att_join<T, DP, true>), dim3((unsigned)rows * (DP / 32)), dim3(256), 0, st, a);
     else
-      hipLaunchKernelGGL((paged_att_join<T, DP, 0>), dim3((unsigned)((rows + kGr - 1) / kGr)), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((paged_att_join<T, DP, false>), dim3((unsigned)((rows + kGr - 1) / kGr)), dim3(256), 0, st, a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
