@@ -97,6 +97,16 @@ def test_attention_c_abi_empty_calls_and_workspace():
     assert lib.mfl_paged_attention_workspace_bytes(_att_args(rows=1, width=1 << 16, max_kv=1 << 20)) > 0
 
 
+def test_attention_c_abi_refuses_a_join_past_the_launch_limit():
+    """Packed rows behind max_rows are joined too (marked as not computed): as many as one launch takes."""
+    lib = nat.load_library()
+    kw = dict(offsets=16, n=1, rows=1, heads=8, kv_heads=8, dim=128, width=1 << 16, max_kv=1 << 20)
+    assert lib.mfl_paged_attention_workspace_bytes(_att_args(total=1 << 20, **kw)) > 0
+    assert lib.mfl_paged_attention_workspace_bytes(_att_args(total=1 << 24, **kw)) == -1
+    assert lib.mfl_paged_attention(_att_args(total=1 << 24, **kw), None) == 1
+    assert b"one launch" in lib.mfl_paged_last_error()
+
+
 # --- pages -------------------------------------------------------------------------------------------
 
 def _upd(**kw):
