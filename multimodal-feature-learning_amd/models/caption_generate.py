@@ -33,6 +33,12 @@ def _grammar(allowed, transitions, vocab, device):
     return allowed.to(device)
 
 
+def _next_state(transitions, state, word):
+    """A state outside the grammar (everything is allowed there) is not left again."""
+    s, last = state.long(), transitions.shape[0] - 1
+    return torch.where((s >= 0) & (s <= last), transitions[s.clamp(0, last), word], state)
+
+
 @torch.no_grad()
 def generate(decoder, prime, step, n, bos, eos, pad, length, device, beams=1, prompt=None, prompt_lens=None,
              repetition=None, presence=None, frequency=None, bias=None, allowed=None, transitions=None,
@@ -94,7 +100,7 @@ def generate(decoder, prime, step, n, bos, eos, pad, length, device, beams=1, pr
         transitions = transitions.to(device=device, dtype=torch.int32)
         for c in range(1, m):  # the prompt's words move the grammar too
             word = captions[:, c].long()
-            state = torch.where(c < at, transitions[state.long(), word], state)
+            state = torch.where(c < at, _next_state(transitions, state, word), state)
     opts = dict(repetition=repetition, presence=presence, frequency=frequency, bias=bias, allowed=allowed)
     live = 1  # beams that hold something
     ends = at.clone()  # words of each caption, the closing <eos> included
@@ -128,7 +134,7 @@ def generate(decoder, prime, step, n, bos, eos, pad, length, device, beams=1, pr
         old = captions.gather(1, idx)
         captions.scatter_(1, idx, torch.where(went[:, None], word[:, None].to(torch.int32), old))
         if transitions is not None:
-            state = torch.where(went, transitions[state.long(), word], state)
+            state = torch.where(went, _next_state(transitions, state, word), state)
         grow = went & (word != pad)
         at = at + went.to(torch.int32)
         ends = torch.where(went, at, ends)

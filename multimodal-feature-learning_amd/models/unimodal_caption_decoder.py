@@ -179,7 +179,7 @@ class UnimodalCaptionDecoder(nn.Module):
         ``process_logits`` (modules/logits.py), over the words so far, <bos> excepted (those of single rows need
         beams = 1).  ``allowed`` (vocab) bool, or a
         grammar: (states, vocab) bool with ``transitions`` (states, vocab), the state after each word, from
-        state 0.  Scores are divided by the number of words ** ``length_penalty`` before the best beam is taken.
+        state 0 (outside [0, states): everything is allowed from then on).  Scores are divided by the number of words ** ``length_penalty`` before the best beam is taken.
         A caption is <bos>, its words, <eos>, then <pad>.  With one beam and no options: greedy_decode's words."""
         mask4 = None if memory_key_mask is None else memory_key_mask[:, None, None, :]
 

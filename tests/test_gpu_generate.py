@@ -154,6 +154,21 @@ def test_grammar(dev, beams):
     assert bool((caps[:, 1] == EOS).all()) and bool((caps[:, 2:] == PAD).all())
 
 
+@pytest.mark.parametrize("beams", [1, 3])
+@pytest.mark.parametrize("outside", [-1, 1, 1 << 30])
+def test_leaving_the_grammar(dev, beams, outside):
+    """A transition to a state that the grammar does not have: everything is allowed from then on."""
+    dec, mems = build("unimodal", seed=8)
+    allowed = torch.zeros(2, V, dtype=torch.bool)
+    allowed[0, 4:20] = allowed[1] = True
+    ones = torch.ones(2, V, dtype=torch.int32)
+    prompt = torch.full((N, 1), 5, dtype=torch.int32)
+    for kw in ({}, {"prompt": prompt}):
+        want = run(dec, mems, dev, beams, allowed=allowed, transitions=ones, **kw)
+        got = run(dec, mems, dev, beams, allowed=allowed[:1], transitions=torch.full_like(ones[:1], outside), **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_prompt_that_fills_the_caption(dev):
     dec, mems = build("unimodal", seed=9)
     prompt = torch.randint(4, V, (N, L - 1), dtype=torch.int32)
