@@ -175,9 +175,9 @@ __device__ __forceinline__ void load_lds_run(const unsigned char* base, const ui
   if constexpr (N == 4)
     asm volatile(
         "s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
-        "global_load_lds_dwordx4 %1, %4 offset:1024\n\tglobal_load_lds_dwordx4 %2, %4 offset:2048\n\t"
-        "global_load_lds_dwordx4 %3, %4 offset:3072" ::"v"(off[0]),
-        "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(dst)
+        "global_load_lds_dwordx4 %1, %4 offset:%6\n\tglobal_load_lds_dwordx4 %2, %4 offset:%7\n\t"
+        "global_load_lds_dwordx4 %3, %4 offset:%8" ::"v"(off[0]),
+        "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(dst), "i"(1024), "i"(2 * 1024), "i"(3 * 1024)
         : "memory", "m0");
   else if constexpr (N == 2)
     asm volatile(
