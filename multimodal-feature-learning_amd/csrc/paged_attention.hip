@@ -8,8 +8,11 @@
 // values' type, are the B operand of O^T += V^T P^T with no movement.  One pass over the keys:
 //   m' = max(m, max_j s_j),  l' = l 2^(c (m - m')) + sum_j 2^(c (s_j - m')),  O' = O 2^(c (m - m')) + P V
 // with c = scale * log2(e); m, l and O stay in fp32 and are rounded once at the end.  P is rounded to the
-// values' 16-bit type for the matrix product (relative 2^-9 / 2^-12 of each weight, against the output's
-// own rounding of the same size); l sums the unrounded weights.
+// values' 16-bit type, the only one that the matrix product takes beside them: at most 2^-8 (bf16) or 2^-11 (fp16)
+// of each weight, as much as the output's own rounding.  l sums the unrounded weights.  fp16 has no such relative
+// bound below its smallest normal number, 2^-14, and nothing below 2^-25: its weights are computed 2^7 times
+// as large (kShift), so that the steps of its subnormal numbers are at most 2^-32 of the largest weight off.  At the weights'
+// true size, 2^17 keys of 2^-25.2 beside one of 1 lose all they add, 7 times the output's rounding.
 //
 // The reference value m follows the maximum only when that has grown by more than 2^8 (any m gives the same
 // quotient): most steps then need no rescale of O and no exchange between lanes.
@@ -452,6 +455,10 @@ __device__ __forceinline__ void mask_scores(f32x16& s, int j0, int lim, uint32_t
 // the online softmax's step for NT score tiles: s replaced by the weights against m; m, l and O rescaled when
 // some row's maximum outgrows m by 2^kLazy.  w.l: the sum of the lane's own scores only
 constexpr float kLazy = 8.f;
+// the weights are 2^kShift times their size, in O and l alike and in every range, so that it drops out of the quotient.
+// fp16: at most 2^(kLazy + kShift) = 2^15, which it holds
+template <class T>
+constexpr float kShift = __is_same(T, _Float16) ? 7.f : 0.f;
 template <class T, int DP, int NT>
 __device__ __forceinline__ void soft_step(Cols<T, DP>& w, f32x16 (&s)[NT], float c) {
   float mx = s[0][0];
@@ -470,7 +477,7 @@ __device__ __forceinline__ void soft_step(Cols<T, DP>& w, f32x16 (&s)[NT], float
 #pragma unroll
       for (int e = 0; e < 16; ++e) w.o[d][e] *= al;
   }
-  const float base = w.m == -INFINITY ? 0.f : w.m * c;  // (nothing seen yet: every weight is 2^-inf = 0)
+  const float base = w.m == -INFINITY ? 0.f : w.m * c - kShift<T>;  // (nothing seen yet: every weight is 2^-inf = 0)
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int t = 0; t < NT; ++t)

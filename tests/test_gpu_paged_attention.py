@@ -11,6 +11,8 @@ keys, A = sum_j p_j |v_j|, S = max_j scale sum_d |q_d k_jd|:
   2^-25 sum_j |v_j|             fp16 only: weights below its smallest normal number, rounded to its steps of 2^-24
                                 (the largest weight is 1, so the denominator is at least 1)
 """
+import math
+
 import pytest
 import torch
 
@@ -383,3 +385,34 @@ def test_chunk_over_key_ranges(dev):
 def test_ways_to_cut_the_keys(dev, n, heads, kvh, dim, rows, kv, dtype):
     d = make(n, rows, heads, kvh, dim, 16, kv, dtype, seed=heads + dim)
     check(call(up(d, dev), max_kv=max(kv)), d)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, F32], ids=["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("bits", [24.5, 25.2, 30.0])
+def test_many_small_weights_beside_a_large_one(dev, rows, bits, dtype):
+    """One key of weight 1 and value 0 beside 32,000 keys of weight 2^-bits and value 1, in one range: the small ones
+    are all that the row's answer is, N w / (1 + N w).
+
+    Tolerance, relative, with u = eps / 2: the output's rounding u; the small weights' rounding u in a 16-bit type (fp16:
+    half a step of its subnormal numbers, 2^-25, of weights computed at 2^7 of their size, 2^(7 - bits): 2^(bits - 32)
+    of each where that is more); 2 w with w = (D + 8) 2^-24 S + 2^-20, S = bits ln 2; 2 K 2^-24 for the sums over K keys."""
+    keys, dim, ps = 32001, 64, 64
+    pages = (keys + ps - 1) // ps
+    k = torch.zeros(pages, 1, ps, dim, dtype=dtype, device=dev)
+    v = torch.ones_like(k)
+    q = torch.zeros(1, rows, 1, dim, dtype=dtype, device=dev)
+    q[..., 0] = 1.0
+    k[0, 0, 0, 0] = 16.0
+    v[0, 0, 0] = 0.0
+    s = bits * math.log(2.0)
+    out = pc.paged_attention(q, k, v, torch.arange(pages, dtype=torch.int32, device=dev)[None],
+                             torch.tensor([keys], dtype=torch.int32, device=dev), scale=s / 16.0, causal=False, max_kv=64)
+    u = torch.finfo(dtype).eps / 2
+    weight = math.exp(-s)
+    want = (keys - 1) * weight / (1.0 + (keys - 1) * weight)
+    rel = u + 2 * ((dim + 8) * 2.0 ** -24 * s + 2.0 ** -20) + 2 * keys * 2.0 ** -24
+    if dtype != F32:
+        rel += max(u, 2.0 ** (bits - 32)) if dtype == FP else u
+    # (an output below fp16's normal numbers is rounded to its steps of 2^-24)
+    assert bool(((out.double() - want).abs() <= rel * want + (2.0 ** -25 if dtype == FP else 0.0)).all())
