@@ -73,7 +73,7 @@ def generate(decoder, prime, step, n, bos, eos, pad, length, device, beams=1, pr
             at = 1 + prompt_lens.to(device=device, dtype=torch.int32).clamp(0, m - 1)
             cols = torch.arange(length, device=device)
             captions.masked_fill_(cols >= at[:, None], pad)
-    if n == 0 or m == length and prompt_lens is None:
+    if n == 0 or length == 1 or m == length and prompt_lens is None:  # no word to pick
         return captions, torch.zeros(n, dtype=torch.float32, device=device)
     cache = PagedCaptionCache(rows, length, page_size, device)
     prime(cache)

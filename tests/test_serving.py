@@ -220,3 +220,25 @@ def test_logits_c_abi_refuses(kw):
     assert lib.mfl_logits_process(_lg_args(**kw), None) == 1
     assert b"mfl_logits_process" in lib.mfl_logits_last_error()
     assert lib.mfl_logits_process(None, None) == 1
+
+
+# --- generate ----------------------------------------------------------------------------------------
+
+def _decoder(vocab=12, d=16):
+    return PKG.models.unimodal_caption_decoder.UnimodalCaptionDecoder(vocab, d_model=d, depth=1, num_heads=2).eval()
+
+
+@pytest.mark.parametrize("beams", [1, 2])
+@pytest.mark.parametrize("length_penalty", [0.0, 0.7])
+def test_generate_without_a_word_to_pick(beams, length_penalty):
+    """Captions of <bos> alone, and prompts that fill them: no decoder pass runs, so the host does."""
+    dec, mem = _decoder(), torch.zeros(3, 5, 16)
+    none = torch.zeros(3, 0, dtype=torch.int32)
+    for kw in (dict(), dict(prompt=none), dict(prompt=none, prompt_lens=_i(3))):
+        caps, scores = dec.generate(mem, None, 2, 3, 1, 1, beams=beams, length_penalty=length_penalty, **kw)
+        assert caps.tolist() == [[2]] * 3 and scores.tolist() == [0.0] * 3
+    caps, scores = dec.generate(mem, None, 2, 3, 1, 3, beams=beams, length_penalty=length_penalty,
+                                prompt=torch.full((3, 2), 5, dtype=torch.int32))
+    assert caps.tolist() == [[2, 5, 5]] * 3 and scores.tolist() == [0.0] * 3
+    caps, scores = dec.generate(mem[:0], None, 2, 3, 1, 4, beams=beams, length_penalty=length_penalty)
+    assert caps.shape == (0, 4) and scores.shape == (0,)
