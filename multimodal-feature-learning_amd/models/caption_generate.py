@@ -47,6 +47,9 @@ def generate(decoder, prime, step, n, bos, eos, pad, length, device, beams=1, pr
     layers on rows x (rows, R, d).  See ``UnimodalCaptionDecoder.generate``."""
     if beams < 1 or length < 1:
         raise ValueError(f"generate: beams {beams}, length {length}")
+    places = decoder.positional_encoding.pos_embedding.shape[1]
+    if length > places:  # (on the device a position behind the table is an assertion, which ends the process)
+        raise ValueError(f"generate: length {length}, the decoder has {places} positions")
     if decoder.training:
         raise RuntimeError("generate: the decoder is in training mode (its dropout would be applied); call eval()")
     vocab = decoder.vocab_size

@@ -242,3 +242,14 @@ def test_generate_without_a_word_to_pick(beams, length_penalty):
     assert caps.tolist() == [[2, 5, 5]] * 3 and scores.tolist() == [0.0] * 3
     caps, scores = dec.generate(mem[:0], None, 2, 3, 1, 4, beams=beams, length_penalty=length_penalty)
     assert caps.shape == (0, 4) and scores.shape == (0,)
+
+
+def test_generate_refuses_captions_past_the_position_table():
+    dec, mem = _decoder(), torch.zeros(3, 5, 16)
+    places = dec.positional_encoding.pos_embedding.shape[1]
+    prompt = torch.full((3, places - 1), 5, dtype=torch.int32)
+    caps, _ = dec.generate(mem, None, 2, 3, 1, places, prompt=prompt)  # (filled by the prompt: nothing runs)
+    assert caps.shape == (3, places)
+    for kw in (dict(), dict(beams=2), dict(prompt=prompt)):
+        with pytest.raises(ValueError, match="positions"):
+            dec.generate(mem, None, 2, 3, 1, places + 1, **kw)
