@@ -33,6 +33,15 @@ def _grammar(allowed, transitions, vocab, device):
     return allowed.to(device)
 
 
+def _words_known(prompt, vocab):
+    """Refuses words outside the vocabulary (on the device an embedding's assertion, which ends the process).  The only
+    wait for the host in ``generate``; a captured call goes without."""
+    if prompt.numel() and not (prompt.is_cuda and torch.cuda.is_current_stream_capturing()):
+        low, high = torch.stack(prompt.aminmax()).tolist()
+        if low < 0 or high >= vocab:
+            raise ValueError(f"generate: prompt words {low} .. {high} of a vocabulary of {vocab}")
+
+
 def _next_state(transitions, state, word):
     """A state outside the grammar (everything is allowed there) is not left again."""
     s, last = state.long(), transitions.shape[0] - 1
@@ -53,6 +62,8 @@ def generate(decoder, prime, step, n, bos, eos, pad, length, device, beams=1, pr
     if decoder.training:
         raise RuntimeError("generate: the decoder is in training mode (its dropout would be applied); call eval()")
     vocab = decoder.vocab_size
+    if not all(0 <= w < vocab for w in (bos, eos, pad)):
+        raise ValueError(f"generate: <bos> {bos}, <eos> {eos} and <pad> {pad} must be among the {vocab} words")
     if beams > vocab:
         raise ValueError(f"generate: {beams} beams over {vocab} words")
     if beams > 1 and (any(isinstance(x, torch.Tensor) for x in (repetition, presence, frequency))
@@ -63,6 +74,10 @@ def generate(decoder, prime, step, n, bos, eos, pad, length, device, beams=1, pr
     if prompt is not None:
         if prompt.dim() != 2 or prompt.shape[0] != n or 1 + prompt.shape[1] > length:
             raise ValueError(f"generate: prompt must be ({n}, at most {length - 1}); got {tuple(prompt.shape)}")
+        if prompt.is_floating_point() or prompt.is_complex():
+            raise ValueError(f"generate: prompt must hold whole numbers; got {prompt.dtype}")
+        if prompt_lens is not None and prompt_lens.shape != (n,):
+            raise ValueError(f"generate: prompt_lens must be ({n},); got {tuple(prompt_lens.shape)}")
         m += prompt.shape[1]
     elif prompt_lens is not None:
         raise ValueError("generate: prompt_lens without prompt")
@@ -71,11 +86,12 @@ def generate(decoder, prime, step, n, bos, eos, pad, length, device, beams=1, pr
     captions[:, 0] = bos
     at = torch.full((n,), m, dtype=torch.int32, device=device)  # the next word's position
     if prompt is not None:
-        captions[:, 1:m] = prompt
+        prompt = prompt.to(device)
         if prompt_lens is not None:
             at = 1 + prompt_lens.to(device=device, dtype=torch.int32).clamp(0, m - 1)
-            cols = torch.arange(length, device=device)
-            captions.masked_fill_(cols >= at[:, None], pad)
+            prompt = prompt.masked_fill(torch.arange(1, m, device=device) >= at[:, None], pad)
+        _words_known(prompt, vocab)
+        captions[:, 1:m] = prompt
     if n == 0 or length == 1 or m == length and prompt_lens is None:  # no word to pick
         return captions, torch.zeros(n, dtype=torch.float32, device=device)
     cache = PagedCaptionCache(rows, length, page_size, device)

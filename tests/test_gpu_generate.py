@@ -239,3 +239,37 @@ def test_the_other_wrappers_with_beams(dev, golden, kind):
         c = model(obj, **kw)
     assert torch.equal(a[1], b[1])
     assert c[1].shape == a[1].shape and bool(torch.isfinite(c[0]['pred_captions']).all())
+
+
+def test_what_stands_behind_a_prompt_does_not_count(dev):
+    """Numbers that are no words behind prompt_lens; words that are none within them are refused before they are looked up."""
+    dec, mems = build("unimodal", seed=7)
+    lens = torch.tensor([3, 2, 1, 0], dtype=torch.int32)
+    prompt = torch.tensor([[5, 6, 7], [8, 9, -1], [10, V, 1 << 20], [-5, 99, V]])
+    clean = torch.tensor([[5, 6, 7], [8, 9, PAD], [10, PAD, PAD], [PAD, PAD, PAD]])
+    for beams in (1, 2):
+        got, want = (run(dec, mems, dev, beams, prompt=p, prompt_lens=lens) for p in (prompt, clean))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        with pytest.raises(ValueError):
+            run(dec, mems, dev, beams, prompt=prompt, prompt_lens=lens + 1)
+
+
+@pytest.mark.parametrize("beams", [1, 3])
+def test_captured_and_replayed(dev, beams):
+    """The whole search as one graph, a prompt included, replayed over other memories."""
+    dec, mems = build("unimodal", seed=7)
+    g = copy.deepcopy(dec).float().to(dev)
+    mem, mask = mems[0].to(dev, torch.float32), mems[1].to(dev)
+    prompt = torch.full((N, 2), 5, dtype=torch.int32, device=dev)
+    call = lambda: g.generate(mem, mask, BOS, EOS, PAD, L, beams=beams, prompt=prompt)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        got = call()
+    for it in range(3):
+        mem.copy_(torch.randn(mem.shape, generator=torch.Generator().manual_seed(it)))
+        want = call()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -253,3 +253,30 @@ def test_generate_refuses_captions_past_the_position_table():
     for kw in (dict(), dict(beams=2), dict(prompt=prompt)):
         with pytest.raises(ValueError, match="positions"):
             dec.generate(mem, None, 2, 3, 1, places + 1, **kw)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(bos=-1), dict(bos=12), dict(eos=-1), dict(eos=12), dict(pad=-1), dict(pad=12),
+    dict(prompt=torch.tensor([[4, 5], [6, 12], [4, 4]])), dict(prompt=torch.tensor([[4, -1], [6, 7], [4, 4]])),
+    dict(prompt=torch.tensor([[4, 5], [6, 7], [4, 2 ** 32 + 4]])), dict(prompt=torch.full((3, 2), 4.0)),
+    dict(prompt=torch.tensor([[4, 99], [6, 7], [4, 4]]), prompt_lens=_i(3) + 2),
+    dict(prompt=torch.full((3, 2), 4), prompt_lens=_i(3, 1)), dict(prompt=torch.full((3, 2), 4), prompt_lens=_i(2))])
+def test_generate_refuses_words_that_are_none(kw):
+    a = dict(bos=2, eos=3, pad=1)
+    a.update(kw)
+    bos, eos, pad = a.pop("bos"), a.pop("eos"), a.pop("pad")
+    for beams in (1, 2):
+        with pytest.raises(ValueError):
+            _decoder().generate(torch.zeros(3, 5, 16), None, bos, eos, pad, 6, beams=beams, **a)
+
+
+def test_words_behind_a_prompt_are_not_looked_at():
+    """A prompt of length 0 whose tensor holds anything, in a caption that it fills."""
+    caps, _ = _decoder().generate(torch.zeros(3, 5, 16), None, 2, 3, 1, 1, prompt=torch.zeros(3, 0, dtype=torch.int64),
+                                  prompt_lens=_i(3))
+    assert caps.tolist() == [[2]] * 3
+    gen = PKG.models.caption_generate
+    words = torch.tensor([[4, -7], [99, 99]])
+    gen._words_known(words.masked_fill(torch.tensor([[False, True], [True, True]]), 1), 12)
+    with pytest.raises(ValueError):
+        gen._words_known(words, 12)
