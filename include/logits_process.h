@@ -9,7 +9,8 @@
  *   x = x + bias[i][v]
  *   x = -inf where the token is not allowed (whatever it was before)
  *   out[i][v] = x  (rounded to out's type),  best[i] = the lowest v of the largest x (NaN counts as the
- *   largest; -1 when every x is -inf),  lse[i] = log sum_v exp(x),  logprob[i] = x[best] - lse (-inf when -1)
+ *   largest; -1 when every x is -inf),  lse[i] = log sum_v exp(x),  logprob[i] = -log sum_v exp(x - x[best])
+ *   (-inf when best is -1, NaN when x[best] is infinite or NaN)
  *
  * logits (n, vocab) rows logits_row elements apart; dtype and out_dtype: 0 float32, 2 bfloat16, 3 float16.  out
  * may be logits itself (same type and stride), else must not overlap it; NULL: not written.  best / lse /

@@ -179,7 +179,9 @@ __device__ __forceinline__ void finish(const Args& a, int row, const Stat& r) {
   else if (top == INFINITY || top == -INFINITY) lse = top;
   if (a.best) a.best[row] = top == -INFINITY ? -1 : (int64_t)(uint32_t)~(uint32_t)r.key;
   if (a.lse) a.lse[row] = lse;
-  if (a.logprob) a.logprob[row] = top == -INFINITY ? -INFINITY : top - lse;
+  // (a finite top is the maximum that the sum is taken against: top - lse without the bits that lse loses to top)
+  const bool finite = top == top && top != INFINITY && top != -INFINITY;
+  if (a.logprob) a.logprob[row] = finite ? 0.f - logf(r.s) : top == -INFINITY ? -INFINITY : NAN;
 }
 
 template <class T, class O, int THREADS, int NCH>

@@ -156,6 +156,7 @@ def process_logits(logits, *, tokens=None, token_lens=None, repetition=None, pre
 def pick_tokens(logits, *, tokens=None, token_lens=None, repetition=None, presence=None, frequency=None, bias=None,
                 allowed=None, states=None):
     """(token (n,) int64, its log-probability (n,) float32) of the logits as ``process_logits`` would leave them,
-    without writing them: the greedy choice (-1 and -inf where nothing is allowed)."""
+    without writing them: the greedy choice (-1 and -inf where nothing is allowed).  The log-probability is summed
+    against the token's own logit, so it keeps its bits however large the logits are."""
     return _run("pick_tokens", logits, tokens, token_lens, repetition, presence, frequency, bias, allowed, states, None,
                 False, True)[1:]

@@ -213,3 +213,43 @@ def test_stream_and_graph(dev):
         for a, b in zip(got, eager):
             assert torch.equal(a, b)
         assert torch.equal(pick[0], eager[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("vocab", [40, 8192, 20001])
+def test_log_probability_of_large_logits(dev, vocab, dtype):
+    """Rows of equal logits have -log V whatever their size, and rows of nearly equal large ones the log-probability of
+    their differences, which fp32 holds exactly.
+
+    Tolerance: the exponentials (differences of at most 2^6, times log2 e: 2^7 u; few ulp: 2^-21) and their sum
+    ((V / 64 + 64) u) relative, so absolute in the logarithm; the logarithm's own 2 u of its value.  Equal logits: the sum
+    is a whole number, exact."""
+    top = torch.finfo(dtype).max
+    for x in (0.0, 1e4, -3e4, top, -top):
+        token, logp = lg.pick_tokens(torch.full((2, vocab), x, dtype=dtype, device=dev))
+        assert token.tolist() == [0, 0]
+        assert bool(((logp.double() + math.log(vocab)).abs() <= 4 * U * math.log(vocab)).all())
+    g = torch.Generator().manual_seed(vocab)
+    for base in (1e2, 1e4, -1e4, 6e4):
+        step = max(2.0 ** -7, torch.finfo(dtype).eps * abs(base))
+        x = (base - step * torch.randint(0, 9, (3, vocab), generator=g)).to(dtype)
+        d = x.double() - x.double().amax(1, keepdim=True)
+        keep = d > -64.0
+        x = torch.where(keep, x, -math.inf)
+        ref = -torch.where(keep, d, -math.inf).exp().sum(1).log()
+        token, logp = lg.pick_tokens(x.to(dev))
+        assert token.tolist() == x.double().argmax(1).tolist()
+        tol = 2 ** 7 * U + 2.0 ** -21 + (vocab / 64 + 64) * U + 4 * U * ref.abs()
+        assert bool(((logp.double().cpu() - ref).abs() <= tol).all())
+
+
+def test_log_probability_without_a_finite_best(dev):
+    x = torch.zeros(4, 20001, device=dev)
+    x[0, 7] = math.inf
+    x[1, 9] = math.nan
+    x[2] = -math.inf
+    x[3] = -math.inf
+    x[3, 20000] = -5.0
+    token, logp = lg.pick_tokens(x)
+    assert token.tolist() == [7, 9, -1, 20000]
+    assert bool(logp[:2].isnan().all()) and float(logp[2]) == -math.inf and float(logp[3]) == 0.0
