@@ -15,7 +15,8 @@
  * logits (n, vocab) rows logits_row elements apart; dtype and out_dtype: 0 float32, 2 bfloat16, 3 float16.  out
  * may be logits itself (same type and stride), else must not overlap it; NULL: not written.  best / lse /
  * logprob may be NULL.  tokens (n, hist) int32, rows tokens_row apart; numbers outside [0, vocab) count nothing;
- * token_lens NULL: hist.  The penalties are per row where a pointer is given, else the scalar.  bias float32,
+ * token_lens NULL: hist.  The penalties are per row where a pointer is given, else the scalar
+ * (repetition: positive and finite in float32).  bias float32,
  * rows bias_row apart (0: one row).  allowed: allowed_kind 1 — bytes, non-zero = allowed; 2 — bits, token v
  * is bit v % 32 of int32 word v / 32; mask rows allowed_row bytes / words apart, allowed_rows of them; row i
  * takes mask row states[i] (outside [0, allowed_rows): everything is allowed), without states row i, or row 0

@@ -381,7 +381,9 @@ bool check(const mfl_logits_args* p) {
   if (p->allowed_kind && p->allowed_rows > 1 &&
       p->allowed_row < (p->allowed_kind == 2 ? (p->vocab + 31) / 32 : p->vocab))
     return bad("%s: mask rows overlap", who);
-  if (!p->repetition_rows && !(p->repetition > 0.0)) return bad("%s: repetition must be positive", who);
+  const float rep = (float)p->repetition;  // (the kernel divides by it)
+  if (!p->repetition_rows && !(rep > 0.f && rep < INFINITY))
+    return bad("%s: repetition must be positive and finite in float32", who);
   if (p->out == p->logits && p->out && (p->dtype != p->out_dtype || (p->n > 1 && p->out_row != p->logits_row)))
     return bad("%s: in place needs one type and stride", who);
   if (p->out && p->n > 1 && p->out_row < p->vocab) return bad("%s: rows of out overlap", who);

@@ -14,6 +14,8 @@ __all__ = ["process_logits", "pick_tokens"]
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 2, torch.float16: 3}
 _ARGS = struct.Struct("=14Q12q3d")  # mfl_logits_args
+# a repetition penalty is divided by in float32, where it must be neither zero nor infinite
+_MIN_REP, _MAX_REP = 2.0 ** -149, torch.finfo(torch.float32).max
 
 
 def _penalty(who, name, x, n, default):
@@ -25,7 +27,7 @@ def _penalty(who, name, x, n, default):
             raise ValueError(f"{who}: {name} must be a number or ({n},) float32; got {tuple(x.shape)} {x.dtype}")
         return x.contiguous(), default
     x = float(x)
-    if x != x or (name == "repetition" and not x > 0.0):
+    if x != x or (name == "repetition" and not _MIN_REP <= x <= _MAX_REP):
         raise ValueError(f"{who}: {name} {x}")
     return None, x
 
@@ -140,7 +142,7 @@ def process_logits(logits, *, tokens=None, token_lens=None, repetition=None, pre
     tokens[i, :token_lens[i]] (int32; numbers outside the vocabulary count nothing), in float32:
       c > 0:  x = x / repetition if x > 0 else x * repetition;  x -= presence;  x -= frequency * c
       x += bias[v] (float32, (vocab,) or (n, vocab));  x = -inf where the token is not allowed
-    ``repetition`` (positive), ``presence``, ``frequency``: numbers or (n,) float32.  ``allowed``: bool, one element a
+    ``repetition`` (positive and finite), ``presence``, ``frequency``: numbers or (n,) float32.  ``allowed``: bool, one element a
     token, or int32, 32 tokens an element (token v is bit v % 32 of element v // 32); one mask row for all, one
     for each row, or any number with ``states`` (n,) int32 choosing row i's (outside the mask rows: everything
     is allowed).

@@ -280,3 +280,17 @@ def test_words_behind_a_prompt_are_not_looked_at():
     gen._words_known(words.masked_fill(torch.tensor([[False, True], [True, True]]), 1), 12)
     with pytest.raises(ValueError):
         gen._words_known(words, 12)
+
+
+@pytest.mark.parametrize("rep", [1e-50, 1e39, float("inf"), -1.0])
+def test_logits_refuse_a_repetition_that_float32_does_not_hold(rep):
+    for f in (lg.process_logits, lg.pick_tokens):
+        with pytest.raises(ValueError):
+            f(torch.zeros(2, 40), tokens=_i(2, 3), repetition=rep)
+    lib = nat.load_library()
+    assert lib.mfl_logits_process(_lg_args(repetition=rep), None) == 1
+    assert b"repetition" in lib.mfl_logits_last_error()
+    for good in (1e-40, 0.5, 1.0, 3e38):
+        with pytest.raises(RuntimeError):  # (host tensors)
+            lg.process_logits(torch.zeros(2, 40), tokens=_i(2, 3), repetition=good)
+        assert lib.mfl_logits_workspace_bytes(_lg_args(repetition=good)) >= 0
