@@ -11,6 +11,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libmsda_hip.so")
@@ -370,6 +371,18 @@ def on_device(index):
 def raw_stream(index):
     """The current stream of device ``index`` as an address."""
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+def inference_only(who, *tensors):
+    """Refuses tensors (None: left out) that a gradient is wanted of, backward or forward: it would be lost."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{who}: inference only (no gradient); call it under torch.no_grad()")
+    if forward_ad._current_level >= 0:  # (within a dual_level; no_grad does not reach forward mode)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{who}: inference only (no forward-mode tangents); pass unpack_dual(t).primal")
 
 
 def device_index(who, named):

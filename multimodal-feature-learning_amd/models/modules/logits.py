@@ -62,8 +62,6 @@ def _run(who, logits, tokens, token_lens, repetition, presence, frequency, bias,
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"{who}: logits must be (n, vocab); got {tuple(logits.shape)}")
     n, vocab = logits.shape
-    if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
-        raise RuntimeError(f"{who}: inference only (no gradient); call it under torch.no_grad()")
     hist = tokens_row = 0
     if tokens is not None:
         if tokens.dim() != 2 or tokens.shape[0] != n:
@@ -83,6 +81,7 @@ def _run(who, logits, tokens, token_lens, repetition, presence, frequency, bias,
     rep_t, rep = _penalty(who, "repetition", repetition, n, 1.0)
     pres_t, pres = _penalty(who, "presence", presence, n, 0.0)
     freq_t, freq = _penalty(who, "frequency", frequency, n, 0.0)
+    _native.inference_only(who, logits, bias, rep_t, pres_t, freq_t, out)
     bias_row = 0
     if bias is not None:
         if bias.dtype != torch.float32:

@@ -113,9 +113,7 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, *, k=None, v=None, star
         want = (total, kvh, d) if packed else (n, rows, kvh, d)
         if k.shape != want or v.shape != want:
             raise ValueError(f"{who}: k / v must be {want}; got {tuple(k.shape)}, {tuple(v.shape)}")
-    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad
-                                    or k is not None and (k.requires_grad or v.requires_grad)):
-        raise RuntimeError(f"{who}: inference only (no gradient); call it under torch.no_grad()")
+    _native.inference_only(who, q, k_pages, v_pages, k, v, out)
     table = _i32(who, "table", table, (n, width))
     kv_lens = _i32(who, "kv_lens", kv_lens, (n,))
     if starts is not None:
@@ -162,6 +160,7 @@ def _data(who, data):
         return 0, 0, 0, 0
     if data.dim() != 6 or data.shape[1] != 2:
         raise ValueError(f"{who}: data must be (layers, 2, pages, kv_heads, page_size, dim); got {tuple(data.shape)}")
+    _native.inference_only(who, data)
     if not data.is_contiguous():
         raise ValueError(f"{who}: data must be contiguous")
     row = data.shape[5] * data.element_size()

@@ -294,3 +294,45 @@ def test_logits_refuse_a_repetition_that_float32_does_not_hold(rep):
         with pytest.raises(RuntimeError):  # (host tensors)
             lg.process_logits(torch.zeros(2, 40), tokens=_i(2, 3), repetition=good)
         assert lib.mfl_logits_workspace_bytes(_lg_args(repetition=good)) >= 0
+
+
+# --- gradients ---------------------------------------------------------------------------------------
+
+def _calls():
+    """Every entry point with each of its tensors that could want a gradient."""
+    f = torch.zeros
+    yield lambda x: _att(q=x), f(2, 3, 4, 64)
+    yield lambda x: _att(k_pages=x), f(5, 2, 16, 64)
+    yield lambda x: _att(v_pages=x), f(5, 2, 16, 64)
+    yield lambda x: _att(k=x, v=f(2, 3, 2, 64)), f(2, 3, 2, 64)
+    yield lambda x: _att(k=f(2, 3, 2, 64), v=x), f(2, 3, 2, 64)
+    yield lambda x: _att(out=x), f(2, 3, 4, 64)
+    yield lambda x: _upd(data=x), f(1, 2, 6, 2, 16, 8)
+    yield lambda x: pc.pages_compact(x, _i(3, 2), _i(6)), f(1, 2, 6, 2, 16, 8)
+    yield lambda x: pc.pages_copy(x, _i(2), _i(2)), f(1, 2, 6, 2, 16, 8)
+    for call in (lg.process_logits, lg.pick_tokens):
+        yield call, f(2, 40)
+        yield lambda x, call=call: call(f(2, 40), bias=x), f(40)
+        for name in ("repetition", "presence", "frequency"):
+            yield lambda x, call=call, name=name: call(f(2, 40), tokens=_i(2, 3), **{name: x}), torch.ones(2)
+    yield lambda x: lg.process_logits(f(2, 40), out=x), f(2, 40)
+
+
+@pytest.mark.parametrize("at", range(20))
+def test_no_gradient_is_lost_without_a_word(at):
+    call, x = list(_calls())[at]
+    with pytest.raises(RuntimeError, match="inference only"):
+        call(x.clone().requires_grad_())
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU implementation"):
+        call(x.clone().requires_grad_())
+    ad = torch.autograd.forward_ad
+    with ad.dual_level():
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="inference only"):
+                call(ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError, match="no CPU implementation"):
+            call(x)
+
+
+def test_every_tensor_is_asked_for_its_gradient():
+    assert len(list(_calls())) == 20
