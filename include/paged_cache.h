@@ -4,7 +4,7 @@
  * built into libmsda_hip.so.
  *
  * A cache of L layers is one buffer `data` (L, 2, pages, kv_heads, page_size, dim): keys at [:, 0],
- * values at [:, 1], page_size a power of two.  Sequence s owns the pages table[s][0 ..] (int32, -1 behind
+ * values at [:, 1], page_size a power of two up to 1024.  Sequence s owns the pages table[s][0 ..] (int32, -1 behind
  * the last one) and lens[s] tokens in them; refs[x] counts the sequences that hold page x (0 = free), so
  * sequences share the pages of a common beginning.
  *

@@ -56,8 +56,8 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, *, k=None, v=None, star
     """Attention of new tokens over a paged cache; a single new token a sequence is the decode step.
 
     q: (n, rows, heads, dim), or packed (total, heads, dim) with ``offsets`` (n + 1) int32: sequence s has the
-    rows offsets[s] .. offsets[s + 1].  k_pages, v_pages: (pages, kv_heads, page_size, dim), page_size a power of two;
-    query head h reads key head h // (heads // kv_heads).  table (n, width) int32: key j of sequence s is row
+    rows offsets[s] .. offsets[s + 1].  k_pages, v_pages: (pages, kv_heads, page_size, dim), page_size a power of two up to
+    1024; query head h reads key head h // (heads // kv_heads).  table (n, width) int32: key j of sequence s is row
     j % page_size of page table[s, j // page_size].  kv_lens (n) int32: cached tokens, the chunk's own included.
     ``starts`` (n) int32: the position of each sequence's first row (default: its rows end the cache).
 
@@ -172,7 +172,8 @@ def _data(who, data):
 def pages_update(data, table, lens, refs, *, parents=None, new_lens=None, page_size=None):
     """The next state of a page pool: every row a share of its parent's pages, cut or grown.
 
-    data: (layers, 2, pages, kv_heads, page_size, dim) or None (``page_size`` then says how long a page is);
+    data: (layers, 2, pages, kv_heads, page_size, dim) or None (``page_size`` then says how long a page is; a power of
+    two up to 1024);
     table (n, width), lens (n), refs (pages), all int32.  Row s of the result holds what row ``parents[s]`` held
     (default: itself; outside [0, n): nothing) up to ``new_lens[s]`` tokens (default: all), and pages for the
     tokens up to new_lens[s] where that is more.  Full pages are shared; a row that grows inside a page that
@@ -286,8 +287,8 @@ class PagedKVCache:
 
     def __init__(self, layers, rows, max_tokens, kv_heads, head_dim, page_size=16, pages=None, dtype=torch.bfloat16,
                  device="cuda"):
-        if page_size < 1 or page_size & (page_size - 1):
-            raise ValueError(f"PagedKVCache: page_size {page_size} is no power of two")
+        if page_size < 1 or page_size > 1024 or page_size & (page_size - 1):
+            raise ValueError(f"PagedKVCache: page_size {page_size} is no power of two up to 1024")
         self.page_size, self.max_tokens = page_size, max_tokens
         width = max(1, (max_tokens + page_size - 1) // page_size)
         pages = rows * width if pages is None else pages  # (no rows can hold more different ones)

@@ -178,6 +178,14 @@ def test_cache_refuses_page_size():
         pc.PagedKVCache(1, 2, 20, 2, 64, page_size=12, device="cpu")
 
 
+@pytest.mark.parametrize("page_size", [0, -16, 2048, 1 << 20])
+def test_cache_refuses_page_sizes_that_its_functions_refuse(page_size):
+    with pytest.raises(ValueError, match="page_size"):
+        pc.PagedKVCache(1, 2, 20, 2, 64, page_size=page_size, device="cpu")
+    for good in (1, 1024):
+        assert pc.PagedKVCache(1, 2, 20, 2, 64, page_size=good, device="cpu").data.shape[4] == good
+
+
 # --- logits ------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("err, kw", [
