@@ -116,7 +116,8 @@ def generate(decoder, prime, step, n, bos, eos, pad, length, device, beams=1, pr
     done = at >= length
     state = torch.zeros(n, dtype=torch.int32, device=device) if allowed is not None else None
     if transitions is not None:
-        transitions = transitions.to(device=device, dtype=torch.int32)
+        # (cut before they are made 32 bits: 2^32 is no state, and must not become 0)
+        transitions = transitions.to(device).clamp(-1, allowed.shape[0]).to(torch.int32)
         for c in range(1, m):  # the prompt's words move the grammar too
             word = captions[:, c].long()
             state = torch.where(c < at, _next_state(transitions, state, word), state)

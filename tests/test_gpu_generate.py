@@ -273,3 +273,17 @@ def test_captured_and_replayed(dev, beams):
         gr.replay()
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("outside", [2 ** 32, -2 ** 32, 2 ** 63 - 1, -2 ** 63])
+def test_transitions_of_64_bits_leave_the_grammar(dev, outside):
+    """States that 32 bits would wrap into the grammar."""
+    dec, mems = build("unimodal", seed=8)
+    allowed = torch.zeros(1, V, dtype=torch.bool)
+    allowed[0, 4:20] = True
+    for beams in (1, 3):
+        want = run(dec, mems, dev, beams, allowed=allowed, transitions=torch.full((1, V), -1))
+        got = run(dec, mems, dev, beams, allowed=allowed, transitions=torch.full((1, V), outside))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    stays = run(dec, mems, dev, 1, allowed=allowed, transitions=torch.zeros(1, V, dtype=torch.int64))
+    assert not torch.equal(stays[0], got[0])  # (leaving the grammar makes a difference here)
