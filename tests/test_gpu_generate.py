@@ -287,3 +287,21 @@ def test_transitions_of_64_bits_leave_the_grammar(dev, outside):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     stays = run(dec, mems, dev, 1, allowed=allowed, transitions=torch.zeros(1, V, dtype=torch.int64))
     assert not torch.equal(stays[0], got[0])  # (leaving the grammar makes a difference here)
+
+
+@pytest.mark.parametrize("kind", ["unimodal", "multimodal"])
+@pytest.mark.parametrize("length", [1, 2, L])
+def test_wrappers_get_the_greedy_outputs_with_one_beam(dev, kind, length):
+    """What the DVC wrappers take from an inference pass, with caption_options and without: the captions, and the
+    decoder's input that pred_captions is computed from."""
+    dec, mems = build(kind, seed=6)
+    g = copy.deepcopy(dec).float().to(dev)
+    args = [t.to(dev, torch.float32) if t.is_floating_point() else t.to(dev) for t in mems]
+
+    vocab = {"<bos>": BOS, "<eos>": EOS, "<pad>": PAD}
+    a = M.dvc_common.decode_captions(g, args, vocab, length, False, None)
+    b = M.dvc_common.decode_captions(g, args, vocab, length, False, dict(beams=1))
+    assert torch.equal(a[0], b[0])
+    assert (a[1] is None) == (b[1] is None) == (length == 1)
+    if length > 1:
+        assert a[1].dtype == b[1].dtype and torch.equal(a[1], b[1])

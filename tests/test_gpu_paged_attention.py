@@ -416,3 +416,24 @@ def test_many_small_weights_beside_a_large_one(dev, rows, bits, dtype):
         rel += max(u, 2.0 ** (bits - 32)) if dtype == FP else u
     # (an output below fp16's normal numbers is rounded to its steps of 2^-24)
     assert bool(((out.double() - want).abs() <= rel * want + (2.0 ** -25 if dtype == FP else 0.0)).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n, rows, heads, kvh, dim, kv", [
+    (112, 2, 8, 8, 64, [1 + i % 19 for i in range(112)]),  # a wave each
+    (3, 1, 8, 2, 128, [4000, 17, 900]),                    # key ranges and their join
+    (2, 70, 4, 2, 64, [1500, 80]),                         # tiles of 128 rows
+], ids=["words", "ranges", "rows"])
+@pytest.mark.parametrize("write", [False, True])
+def test_repeats_itself_exactly(dev, n, rows, heads, kvh, dim, kv, dtype, write):
+    """The same call again, over pages that already hold the chunk and over fresh ones: bit for bit the same."""
+    kv = [max(x, rows) for x in kv]
+    d = make(n, rows, heads, kvh, dim, 16, kv, dtype, seed=n + dim, write=write)
+    g = up(d, dev)
+    first = call(g, max_kv=max(kv))
+    pages = g["k_pages"].clone(), g["v_pages"].clone()
+    for _ in range(5):
+        h = up(d, dev)
+        assert torch.equal(call(h, max_kv=max(kv)), first) and torch.equal(call(g, max_kv=max(kv)), first)
+        for a, b in ((h["k_pages"], pages[0]), (h["v_pages"], pages[1]), (g["k_pages"], pages[0])):
+            assert torch.equal(a.nan_to_num(7.25), b.nan_to_num(7.25))
