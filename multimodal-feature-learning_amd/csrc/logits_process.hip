@@ -12,8 +12,10 @@
 // tiles' (key, sum of exponentials) pairs.
 //
 // Measured on one MI355X: 256 x 128,005 fp32 to fp32 with statistics, packed masks of 40 states, a bias and
-// histories of up to 4,096: 70 us (3.8 TB/s), of which the histories are 20, the masks 6 and the bias 5; with tiles
-// of 4,096 tokens 6 us more.  112 x 10,000 bf16, pick only: 8 us in one tile a row, 6 + 3 us in five and a join.
+// histories of up to 4,096: 70 us in logits_tile (3.8 TB/s) and 5 in logits_join, 77 to 80 a call; the histories are
+// 20 of it, the masks 6 and the bias 5; with tiles of 4,096 tokens 6 us more.  While a workgroup counts and applies its
+// history none of its logits are in flight, and each of a row's 16 tiles reads the history again.  112 x 10,000
+// bf16, pick only: 8 us in one tile a row, 6 + 3 us in five and a join.
 // Loads come before the history's phases: the bias fetched behind them cost 25 us of the large case.
 //
 // The arithmetic is the header's, operation by operation: contraction is off, so that equal logits stay

@@ -24,18 +24,21 @@
 //
 // Keys and values go to LDS by global_load_lds (16 bytes a lane): no registers are held while the loads fly,
 // so a wave keeps 16 to 32 KB in flight, and the rows of up to four loads that lie in one page have one
-// scalar address.
+// scalar address.  Two classes of calls have less: fp32 wider than 64, whose tile of 32 KB is the whole ring (its loads
+// fly between the steps, not beside them), and pages of fewer than 16 tokens (8 in fp32 wider than 64) or widths
+// other than 32, 64 and 128, whose loads have an address a lane (load_tile).
 //
 // Measured on one MI355X (a 1 GB copy moves 5.0 TB/s, an 8192^3 product runs at 1.19 PFLOP/s in bf16, 154 TFLOP/s
-// in fp32):
-//   24 single tokens over 1 .. 16,384 keys, 32 / 8 heads of 128, bf16: 178 us, 5.1 TB/s — the memory's rate
-//   one single token over 131,071 keys, 16 / 2 heads of 128, fp16: 31 us (4.3 TB/s; 5 us of it the join)
-//   2 x 4,096 rows over 6,001 / 12,288 keys, 32 / 8 heads of 128, bf16: 970 us, 0.98 PFLOP/s.  A wave's step of 64
-//   keys takes the matrix unit 1,024 cycles and the vector unit some 1,130 (32 exponentials a lane at a
-//   quarter of the rate); with two waves a SIMD they overlap in part.  Not the loads' bandwidth (the same tile
-//   loaded again and again takes as long; 96 % come from the L2), but issuing them was 9 % until runs shared an
-//   address.  Priorities for the matrix products, 8 waves a tile, rings of 3 and 4, steps of 32 and 128 keys, and
-//   a pipeline over steps (Q K of the next and P V of the last beside this one's exponentials) measured
+// in fp32), us a call:
+//   24 single tokens over 1 .. 16,384 keys, 32 / 8 heads of 128, bf16: 178, 5.1 TB/s — the memory's rate.  fp32 467
+//   (3.9 TB/s); bf16 in pages of 8 tokens 209, at width 96 204 (3.4 TB/s of what it needs), fp32 at width 96 629
+//   one single token over 131,071 keys, 16 / 2 heads of 128, fp16: 35 (3.9 TB/s); the kernels take 26 + 5
+//   2 x 4,096 rows over 6,001 / 12,288 keys, 32 / 8 heads of 128, bf16: 965, 0.99 PFLOP/s.  A wave's step of 64
+//   keys takes the matrix unit 1,024 cycles and the vector unit some 1,000 (214 instructions, 32 of them matrix products
+//   and 32 exponentials at a quarter of the rate); with two waves a SIMD they overlap in part.  Not the loads' bandwidth
+//   (the same tile loaded again and again takes as long; 96 % come from the L2), but issuing them was 9 % until runs
+//   shared an address.  Priorities for the matrix products, 8 waves a tile, rings of 3 and 4, steps of 32 and 128 keys,
+//   and a pipeline over steps (Q K of the next and P V of the last beside this one's exponentials) measured
 //   the same or slower: what they gain in overlap they lose in registers, and with them in waves.
 //
 // MFMA 32x32x16 (16-bit): A lane (h, r): row r = lane & 31, k 8h..8h+7 (h = lane >> 5); B the same with
@@ -241,7 +244,8 @@ struct Pages {
 // loads of 1 KB (64 lanes) for image rows r0 .. of keys j0 + r0 ..: IT of them for keys and values each, LDS images
 // at kd and vd.  `safe`: keys below it come from the pages and are there.  Where up to 16 rows lie in one page
 // (and a row has all DP columns) the run of their loads has one scalar address: what this loop issues
-// beside the loads is a third of a step's instructions otherwise
+// beside the loads is a third of a step's instructions otherwise.  The other branch takes every tile that holds one of the
+// chunk's own keys, and all tiles of smaller pages and other widths
 template <class T, int DP, int IT>
 __device__ __forceinline__ void load_tile(const Args& a, const Seq& q, const Pages& pg, const unsigned char* kn,
                                           const unsigned char* vn, int kh, int j0, int r0, int safe, uint32_t kd,
@@ -726,7 +730,9 @@ __device__ __forceinline__ Range range_of(const Args& a, int most, int split, in
   return r;
 }
 
-// (two waves a SIMD: left to itself the compiler keeps O in accumulation registers, and one wave fits at DP = 128)
+// (two waves a SIMD: left to itself the compiler keeps O in accumulation registers, and one wave fits at DP = 128.  The
+// two-wave form's 64 KB of tiles let two workgroups run on a CU, one wave a SIMD, and its registers, 185 + 80 at DP = 128,
+// allow no more.  All instances keep 18 to 31 scalars in lanes of a vector register; nothing goes to memory)
 template <class T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 1 ? 2 : 1) void paged_att_split(Args a) {
   typedef Geo<T, DP> Ge;

@@ -6,7 +6,8 @@ with dense cached rows.  ``generate`` adds prompts, beams, penalties, biases and
 word is the same — its probabilities are the output row of a <pad> probe at its position, over the keys of the
 committed words that are not <pad> — but the words' keys and values live in pages (modules/paged_cache.py): a
 prompt enters as one chunk, beams share the pages of their common beginning, and a beam that dies frees its
-own.  With one beam and no options it picks greedy_decode's words.  No host synchronisation inside the loop."""
+own.  With one beam and no options it picks greedy_decode's words.  No host synchronisation inside the loop; a
+prompt's words are checked before it."""
 import torch
 
 from .modules.layers import PagedCaptionCache
@@ -123,7 +124,7 @@ def generate(decoder, prime, step, n, bos, eos, pad, length, device, beams=1, pr
             state = torch.where(c < at, _next_state(transitions, state, word), state)
     opts = dict(repetition=repetition, presence=presence, frequency=frequency, bias=bias, allowed=allowed)
     live = 1  # beams that hold something
-    ends = at.clone()  # words of each caption, the closing <eos> included
+    ends = at.clone()  # length of each caption: <bos>, the prompt and the closing <eos> included
     picks = length - (m if prompt_lens is None else 1)  # of the shortest prompt
     for left in range(picks - 1, -1, -1):
         if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):

@@ -146,7 +146,8 @@ def process_logits(logits, *, tokens=None, token_lens=None, repetition=None, pre
     for each row, or any number with ``states`` (n,) int32 choosing row i's (outside the mask rows: everything
     is allowed).
 
-    Returns ``out`` (n, vocab), float32 unless one is given (``out=logits`` works in place); with ``stats``
+    Returns ``out`` (n, vocab), float32 unless one is given (``out=logits`` works in place; other memory must be apart
+    from the logits'); with ``stats``
     (out, best, lse): the best token (n,) int64 — the lowest of equals, NaN above all, -1 when nothing is
     left — and the log-sum-exp (n,) float32 of the values before they are rounded to out's type."""
     res = _run("process_logits", logits, tokens, token_lens, repetition, presence, frequency, bias, allowed, states, out,

@@ -66,8 +66,9 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, *, k=None, v=None, star
     row i's are written to the pages at p, where p is in [0, kv_lens), and attended.  The positions written must
     lie in pages that no other sequence reads (``pages_update`` sees to it).
 
-    ``max_rows``: the largest number of rows of a packed sequence (rows beyond it are neither computed nor written;
-    default: total).  ``max_kv`` guides the launch only (default: what the table holds).  ``scale``: dim ** -0.5.
+    ``max_rows``: the largest number of rows of a packed sequence (rows beyond it are neither computed nor written: what
+    a new tensor holds there is undefined; default: total).  ``max_kv`` guides the launch only (default: what the table
+    holds).  ``scale``: dim ** -0.5.
     Returns ``out``, q's shape and type, contiguous; packed rows before the first sequence and behind the last are
     0 in a new tensor and stay as they were in a given one.  float32, bfloat16 and float16; dim up to 128, a multiple of
     16 bytes; float32 statistics.  No gradients.
@@ -299,7 +300,8 @@ class PagedKVCache:
         self.short = torch.zeros(1, dtype=torch.int32, device=device)
 
     def update(self, parents=None, new_lens=None):
-        """``pages_update`` of the whole cache."""
+        """``pages_update`` of the whole cache.  The state becomes new tensors: a captured update reads those of its
+        capture at every replay, so steps that follow each other copy the results back into them (or are one graph)."""
         self.table, self.lens, self.refs, self.short = pages_update(
             self.data, self.table, self.lens, self.refs, parents=parents, new_lens=new_lens)
 

@@ -173,14 +173,17 @@ class UnimodalCaptionDecoder(nn.Module):
 
     def generate(self, memory, memory_key_mask, bos, eos, pad, length, beams=1, **options):
         """Captions by beam search from a paged cache: (captions (N, ``length``) int32, scores (N) float32, the sum of
-        the words' log-probabilities).  memory (N, K, d), memory_key_mask (N, K) bool (True = masked) or None.
-        ``beams`` captions a sequence; ``prompt`` (N, words) int words that every caption begins with after <bos>
-        (prompt_lens (N): how many of them; no <pad> among them); ``repetition``, ``presence``, ``frequency``, ``bias``: of
-        ``process_logits`` (modules/logits.py), over the words so far, <bos> excepted (those of single rows need
-        beams = 1).  ``allowed`` (vocab) bool, or a
-        grammar: (states, vocab) bool with ``transitions`` (states, vocab), the state after each word, from
-        state 0 (outside [0, states): everything is allowed from then on).  Scores are divided by the number of words ** ``length_penalty`` before the best beam is taken.
-        A caption is <bos>, its words, <eos>, then <pad>.  With one beam and no options: greedy_decode's words."""
+        the words' log-probabilities).  memory (N, K, d), memory_key_mask (N, K) bool (True = masked) or None; length
+        at most the position table's.  ``beams`` captions a sequence; ``prompt`` (N, words) int words that every caption
+        begins with after <bos> (prompt_lens (N): how many of them; no <pad> among them); ``repetition``, ``presence``,
+        ``frequency``, ``bias``: of ``process_logits`` (modules/logits.py), over the words so far, <bos> excepted (those
+        of single rows need beams = 1).  ``allowed`` (vocab) bool, or a grammar: (states, vocab) bool with
+        ``transitions`` (states, vocab), the state after each word, from state 0 (outside [0, states): everything is
+        allowed from then on).  Before the best beam is taken its score is divided by the caption's length **
+        ``length_penalty``; <bos>, the prompt and <eos> count in it, though only the words behind the prompt have scores.
+        A caption is <bos>, its words, <eos>, then <pad>.  With one beam and no options: greedy_decode's words, but where
+        two are as likely as each other to within rounding.  The call may be captured into a graph (a prompt's words are
+        then not checked against the vocabulary)."""
         mask4 = None if memory_key_mask is None else memory_key_mask[:, None, None, :]
 
         def prime(cache):
