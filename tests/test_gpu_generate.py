@@ -305,3 +305,34 @@ def test_wrappers_get_the_greedy_outputs_with_one_beam(dev, kind, length):
     assert (a[1] is None) == (b[1] is None) == (length == 1)
     if length > 1:
         assert a[1].dtype == b[1].dtype and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("amp", [False, True])
+def test_captured_over_a_large_vocabulary(dev, amp):
+    """A vocabulary over which the library's choice of the beams takes several workgroups a row, with penalties, a bias and
+    a grammar of one state; every replay over other memories, eager calls between."""
+    torch.manual_seed(3)
+    vocab, n, length = 10000, 6, 8
+    dec = M.unimodal_caption_decoder.UnimodalCaptionDecoder(vocab, d_model=64, depth=2, num_heads=2).eval().to(dev)
+    with torch.no_grad():
+        dec.head.weight.mul_(20.0)
+    mem = torch.randn(n, 15, 64, device=dev)
+    allowed = torch.rand(vocab, device=dev) < 0.8
+    bias = torch.randn(vocab, device=dev)
+    kw = dict(beams=4, repetition=1.3, presence=0.2, bias=bias, allowed=allowed, length_penalty=0.5)
+
+    def call():
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=amp, cache_enabled=False):
+            return dec.generate(mem, None, BOS, EOS, PAD, length, **kw)
+
+    call()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        got = call()
+    for it in range(4):
+        mem.copy_(torch.randn(mem.shape, generator=torch.Generator().manual_seed(it)))
+        want = call()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), it
