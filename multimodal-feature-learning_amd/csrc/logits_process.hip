@@ -181,7 +181,7 @@ __device__ __forceinline__ void finish(const Args& a, int row, const Stat& r) {
   else if (top == INFINITY || top == -INFINITY) lse = top;
   if (a.best) a.best[row] = top == -INFINITY ? -1 : (int64_t)(uint32_t)~(uint32_t)r.key;
   if (a.lse) a.lse[row] = lse;
-  // (a finite top is the maximum that the sum is taken against: top - lse without the bits that lse loses to top)
+  // (a finite top is the maximum that the sum is taken against: -log s has the bits that top - lse would lose to top)
   const bool finite = top == top && top != INFINITY && top != -INFINITY;
   if (a.logprob) a.logprob[row] = finite ? 0.f - logf(r.s) : top == -INFINITY ? -INFINITY : NAN;
 }
